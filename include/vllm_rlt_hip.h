@@ -49,6 +49,9 @@
  *   vrh_scatter_rows         kernels/routing.py:69-83 (scatter_kernel)
  *   vrh_gather_segments      kernels/routing.py:86-113 (gather_segments_kernel)
  *   vrh_scatter_segments     kernels/routing.py:116-144 (scatter_segments_kernel)
+ *   vrh_sequence_metadata    (none: the host builder is worker/metadata.py:21-68)
+ *   vrh_kv_append_q8, vrh_kv_read_q8, vrh_paged_decode_q8, vrh_paged_prefill_q8
+ *                            (none: an 8-bit cache, see their declarations)
  *   vrh_silu_and_mul         csrc/activation/silu_and_mul.cu:221-245 (silu_and_mul_cuda),
  *                            kernels/activation.py:20-33 (its Torch contract)
  */
@@ -321,6 +324,108 @@ int vrh_routing_metadata(const int64_t* descriptors, const int32_t* tables, int6
 /* slots[r] = r < n ? descriptors[r * 3] : 0 for r < size. */
 int vrh_routing_slots(const int64_t* descriptors, int64_t* slots, int64_t n, int64_t size,
                       vrh_stream_t stream);
+
+/* A packed step's metadata from lengths on the GPU, in one launch. Request r of n has
+ * table row table_rows[r] and, after the step, context_lengths[r] tokens of which the
+ * last query_lengths[r] are new; its tokens follow those of request r - 1:
+ *   cu_seqlens_q[r + 1] = cu_seqlens_q[r] + query_lengths[r], cu_seqlens_q[0] = 0
+ *   out_tables[r, c] = c < ceil(length / page) ? tables[table_rows[r], c] : -1
+ *   out_lengths[r] = context_lengths[r]
+ * and for token t < tokens of request r, i = t - cu_seqlens_q[r]:
+ *   positions[t] = context_lengths[r] - query_lengths[r] + i, write_mask[t] = 1
+ *   write_blocks[t] = tables[table_rows[r], positions[t] / page]
+ *   write_offsets[t] = positions[t] % page
+ * Tokens behind the last request's get 0 everywhere. Lengths are cut to what fits:
+ * negative ones to 0, query lengths to the context, contexts to min(width, out_width)
+ * * page tokens, and new tokens past `tokens` are dropped with their context. A
+ * table_rows[r] outside [0, num_rows) is a request of length 0. */
+int vrh_sequence_metadata(const int32_t* tables, int64_t num_rows, int64_t table_stride,
+                          const int64_t* table_rows, const int32_t* context_lengths,
+                          const int32_t* query_lengths, int64_t* positions, int64_t* write_blocks,
+                          int64_t* write_offsets, uint8_t* write_mask, int32_t* out_tables,
+                          int64_t out_table_stride, int32_t* out_lengths, int32_t* cu_seqlens_q,
+                          int64_t n, int64_t tokens, int32_t width, int32_t out_width,
+                          int32_t page, vrh_stream_t stream);
+
+/* ============================================================== 8-bit cache
+ * K and V as e4m3 bytes [num_blocks, block_size, kv_heads, head_dim] per layer, both
+ * with the same strides (head_dim contiguous, any order of the others), and
+ * scales [num_blocks, kv_heads, 2] bytes (the last dimension contiguous): for each
+ * block of tokens and KV head the biased exponents e of K's and of V's scale. A byte
+ * stands for e4m3 * 2^(e - 127). Cache strides are in bytes, scale strides too; a
+ * layer of a pool is a base pointer, as above. Block tables, lengths and
+ * cu_seqlens_q are those of the 16-bit entry points. Page ids outside
+ * [0, num_blocks) are never used as addresses: appends to them write nothing, reads
+ * of them give zeros, attention reads some block of the pool instead.
+ *
+ * append: sequence s holds context_lengths[s] tokens after the call, its last
+ * cu_seqlens_q[s + 1] - cu_seqlens_q[s] new (one without cu_seqlens_q, then total_q ==
+ * num_seqs; a length of 0 appends nothing): rows cu_seqlens_q[s] .. of k and v. Per
+ * page with a new token, KV head, and K and V apart, a = max |x| over the page's new
+ * finite values:
+ *   e' = the least e >= 27 with a <= 448 * 2^(e - 127)
+ *   e = the page holds older tokens of the sequence ? max(e', its exponent) : e'
+ *   new byte = e4m3(x * 2^(127 - e)), older byte = e4m3(e4m3 * 2^(e_old - e))
+ * rounded to nearest even; NaN and infinities become NaN. Bytes behind a sequence's
+ * last token are left. A page belongs to one of the call's sequences (a shared page
+ * is copied first). */
+int vrh_kv_append_q8(int dtype, void* key_cache, void* value_cache, void* scales,
+                     int64_t cache_block_stride, int64_t cache_token_stride,
+                     int64_t cache_head_stride, int64_t scale_block_stride,
+                     int64_t scale_head_stride, const void* k, const void* v,
+                     int64_t k_row_stride, int64_t k_head_stride, int64_t v_row_stride,
+                     int64_t v_head_stride, const int32_t* block_tables,
+                     const int32_t* context_lengths, const int32_t* cu_seqlens_q,
+                     int64_t num_seqs, int64_t total_q, int32_t kv_heads, int32_t head_dim,
+                     int64_t num_blocks, int32_t block_size, int32_t table_width,
+                     int64_t table_stride, vrh_stream_t stream);
+
+/* out[i, t, h, d] = the value of block pages[i], rounded to the dtype; out is
+ * contiguous [num_pages, block_size, kv_heads, head_dim]. */
+int vrh_kv_read_q8(int dtype, void* out_k, void* out_v, const void* key_cache,
+                   const void* value_cache, const void* scales, int64_t cache_block_stride,
+                   int64_t cache_token_stride, int64_t cache_head_stride,
+                   int64_t scale_block_stride, int64_t scale_head_stride, const int64_t* pages,
+                   int64_t num_pages, int32_t kv_heads, int32_t head_dim, int64_t num_blocks,
+                   int32_t block_size, vrh_stream_t stream);
+
+/* vrh_paged_decode over the 8-bit cache: q and out of `dtype`, head_dim <= 256. The
+ * workspace (NULL where its size is 0) needs no initialisation. A row's result depends
+ * only on that row. */
+size_t vrh_paged_decode_q8_workspace_bytes(int64_t rows, int32_t q_heads, int32_t head_dim,
+                                           int32_t block_size, int32_t table_width,
+                                           int32_t window);
+int vrh_paged_decode_q8(int dtype, void* out, const void* q, const void* key_cache,
+                        const void* value_cache, const void* scales, const int32_t* block_tables,
+                        const int32_t* context_lengths, int64_t rows, int32_t q_heads,
+                        int32_t kv_heads, int32_t head_dim, int64_t num_blocks,
+                        int32_t block_size, int32_t table_width, int64_t table_stride,
+                        int64_t q_row_stride, int64_t q_head_stride, int64_t out_row_stride,
+                        int64_t out_head_stride, int64_t cache_block_stride,
+                        int64_t cache_token_stride, int64_t cache_head_stride,
+                        int64_t scale_block_stride, int64_t scale_head_stride, int32_t window,
+                        void* workspace, size_t workspace_bytes, vrh_stream_t stream);
+
+/* vrh_paged_prefill over the 8-bit cache. Rows of q outside [cu_seqlens_q[0],
+ * cu_seqlens_q[num_seqs]) belong to no sequence and their output is left. With
+ * max_seqlen_q <= 8 every query equals, bit for bit, vrh_paged_decode_q8 of a row with
+ * its length. */
+size_t vrh_paged_prefill_q8_workspace_bytes(int64_t num_seqs, int64_t total_q,
+                                            int32_t max_seqlen_q, int32_t q_heads,
+                                            int32_t kv_heads, int32_t head_dim,
+                                            int32_t block_size, int32_t table_width);
+int vrh_paged_prefill_q8(int dtype, void* out, const void* q, const void* key_cache,
+                         const void* value_cache, const void* scales,
+                         const int32_t* block_tables, const int32_t* context_lengths,
+                         const int32_t* cu_seqlens_q, int64_t num_seqs, int64_t total_q,
+                         int32_t max_seqlen_q, int32_t q_heads, int32_t kv_heads,
+                         int32_t head_dim, int64_t num_blocks, int32_t block_size,
+                         int32_t table_width, int64_t table_stride, int64_t q_token_stride,
+                         int64_t q_head_stride, int64_t out_token_stride,
+                         int64_t out_head_stride, int64_t cache_block_stride,
+                         int64_t cache_token_stride, int64_t cache_head_stride,
+                         int64_t scale_block_stride, int64_t scale_head_stride,
+                         void* workspace, size_t workspace_bytes, vrh_stream_t stream);
 
 #ifdef __cplusplus
 }

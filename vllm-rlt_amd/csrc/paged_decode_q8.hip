@@ -1,0 +1,398 @@
+// Paged single-query (decode) attention over the 8-bit cache (format: q8.h).
+//
+// out[r, h] = softmax_t(q[r, h] . K_t / sqrt(D)) V_t over the visible tokens t of row
+// r, K_t = e4m3 * 2^(ek - 127) of t's page and KV head h / group, V_t likewise.
+//
+// One pass over the keys with the running maximum and sum of the softmax; a row's
+// keys are cut into splits of whole pages whose (max, sum, accumulator) are merged
+// in split order. The cut depends on the row's own length only, so a row's result
+// does not depend on the batch, and a packed query equals a decode row bit for bit.
+#include <algorithm>
+#include <type_traits>
+
+#include "decode_q8.h"
+
+namespace vrh {
+namespace {
+
+// Tokens of the shortest split, and the most splits of a row.
+constexpr int kSplitTokens = 128;
+constexpr int kMaxSplitsQ8 = 32;
+
+struct PartitionQ8 {
+  int start;   // first visible token
+  int first;   // first page
+  int pages;   // pages touched
+  int bps;     // pages per split
+  int nsplit;
+};
+
+__device__ __forceinline__ PartitionQ8 partition_q8(int n, const DecodeQ8Args& a) {
+  PartitionQ8 p;
+  p.start = (a.d.window > 0 && n > a.d.window) ? n - a.d.window : 0;
+  if (a.d.bs_shift >= 0) {
+    p.first = p.start >> a.d.bs_shift;
+    p.pages = ((n - 1) >> a.d.bs_shift) + 1 - p.first;
+  } else {
+    p.first = p.start / a.d.block_size;
+    p.pages = (n - 1) / a.d.block_size + 1 - p.first;
+  }
+  p.bps = max(a.d.min_bps, ceil_div(p.pages, a.slots));
+  p.nsplit = ceil_div(p.pages, p.bps);
+  return p;
+}
+
+// ------------------------------------------------------ any shape, VALU
+// One wave per (split, q head, row). LPT lanes cover a token's head_dim with VE
+// elements each (ND vectors of VE, LPT * VE apart, where that is not enough), so a
+// wave load covers 64 / LPT tokens; U such loads of K and of V are issued back to
+// back. Each token group keeps its own softmax state, merged once per split. All
+// arithmetic is fp32: float32 queries, and every shape the matrix kernel does not take.
+template <typename T, int VE, int LPT, int ND>
+__global__ __launch_bounds__(64) void paged_decode_q8_kernel(DecodeQ8Args a) {
+  constexpr int U = VE >= 4 ? 4 : 2;
+  constexpr int TPL = 64 / LPT;
+  constexpr int CH = U * TPL;
+  using raw_t = raw_of<VE>;
+  const int lane = threadIdx.x;
+  const int dg = lane % LPT, tg = lane / LPT;
+  const int head = blockIdx.y;
+  const int kvh = head / a.d.group;
+  const int64_t row = a.d.row_base + blockIdx.z;
+  int64_t trow, qrow;
+  const int n = row_length(row, a.d, &trow, &qrow);
+  if (n < 0) return;
+  T* out = reinterpret_cast<T*>(a.d.out) + qrow * a.d.o_row + (int64_t)head * a.d.o_head;
+  if (n == 0) {
+    if (blockIdx.x == 0)
+      for (int d = lane; d < a.d.head_dim; d += 64) out[d] = from_f32<T>(0.f);
+    return;
+  }
+  const PartitionQ8 P = partition_q8(n, a);
+  const int split = blockIdx.x;
+  if (split >= P.nsplit) return;
+
+  float qf[ND][VE], acc[ND][VE];
+  int dim[ND];  // this lane's dims, clamped into the row (their q is zero, they store nothing)
+  bool dvalid[ND];
+  const T* qp = reinterpret_cast<const T*>(a.d.q) + qrow * a.d.q_row + (int64_t)head * a.d.q_head;
+#pragma unroll
+  for (int j = 0; j < ND; ++j) {
+    const int d0 = (j * LPT + dg) * VE;
+    dvalid[j] = d0 < a.d.head_dim;
+    dim[j] = dvalid[j] ? d0 : 0;
+#pragma unroll
+    for (int i = 0; i < VE; ++i) {
+      qf[j][i] = dvalid[j] ? to_f32(qp[dim[j] + i]) * a.d.scale_log2 : 0.f;
+      acc[j][i] = 0.f;
+    }
+  }
+  const uint8_t* kbase = reinterpret_cast<const uint8_t*>(a.d.k) + (int64_t)kvh * a.d.k_head;
+  const uint8_t* vbase = reinterpret_cast<const uint8_t*>(a.d.v) + (int64_t)kvh * a.d.v_head;
+  const uint8_t* sbase = a.scales + (int64_t)kvh * a.s_head;
+  const int32_t* table = a.d.tables + trow * a.d.table_stride;
+  const int s0 = P.first + split * P.bps, s1 = min(s0 + P.bps, P.first + P.pages);
+  float m = -INFINITY, l = 0.f;
+
+  for (int seg = s0; seg < s1; seg += 64) {
+    // Up to 64 page ids and their scales, one page a lane.
+    const int seg1 = min(s1, seg + 64);
+    const int blk = seg + lane < seg1 ? pool_block(table[seg + lane], a) : 0;
+    const uint32_t ex = q8_exponents(sbase + (int64_t)blk * a.s_block);
+    // (int64: the last page's end may lie past 2^31 tokens)
+    const int tb = max(P.start, seg * a.d.block_size);
+    const int te = (int)min((int64_t)n, (int64_t)seg1 * a.d.block_size);
+    for (int left = te - tb; left > 0; left -= CH) {
+      const int p0 = te - left;
+      raw_t kr[U][ND], vr[U][ND];
+      float ks[U], vs[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        // Positions past the end read the last token again (and are masked).
+        const int pos = left > u * TPL + tg ? p0 + u * TPL + tg : te - 1;
+        int page, off;
+        if (a.d.bs_shift >= 0) {
+          page = pos >> a.d.bs_shift;
+          off = pos & (a.d.block_size - 1);
+        } else {
+          page = pos / a.d.block_size;
+          off = pos - page * a.d.block_size;
+        }
+        const int64_t b = shfl_i32(blk, page - seg);
+        const uint32_t e = (uint32_t)shfl_i32((int)ex, page - seg);
+        ks[u] = q8_scale(e & 255);
+        vs[u] = q8_scale(e >> 8);
+#pragma unroll
+        for (int j = 0; j < ND; ++j) {
+          kr[u][j] = __builtin_nontemporal_load(reinterpret_cast<const raw_t*>(
+              kbase + b * a.d.k_block + (int64_t)off * a.d.k_token + dim[j]));
+          vr[u][j] = __builtin_nontemporal_load(reinterpret_cast<const raw_t*>(
+              vbase + b * a.d.v_block + (int64_t)off * a.d.v_token + dim[j]));
+        }
+      }
+      float sc[U], mx = m;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        float d = 0.f;
+#pragma unroll
+        for (int j = 0; j < ND; ++j) {
+          float x[VE];
+          q8_values<VE>(kr[u][j], x);
+#pragma unroll
+          for (int i = 0; i < VE; ++i) d = fmaf(qf[j][i], x[i], d);
+        }
+        d = group_sum<LPT>(d) * ks[u];
+        sc[u] = left > u * TPL + tg ? d : -INFINITY;
+        mx = fmaxf(mx, sc[u]);
+      }
+      const float safe = mx == -INFINITY ? 0.f : mx;
+      const float corr = fast_exp2(m - safe);
+      l *= corr;
+#pragma unroll
+      for (int j = 0; j < ND; ++j)
+#pragma unroll
+        for (int i = 0; i < VE; ++i) acc[j][i] *= corr;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float p = fast_exp2(sc[u] - safe);
+        l += p;
+        const float w = p * vs[u];
+        // A masked token's weight is 0, and its value must not matter (0 * NaN).
+        const bool seen = left > u * TPL + tg;
+#pragma unroll
+        for (int j = 0; j < ND; ++j) {
+          float x[VE];
+          q8_values<VE>(vr[u][j], x);
+#pragma unroll
+          for (int i = 0; i < VE; ++i) acc[j][i] = seen ? fmaf(w, x[i], acc[j][i]) : acc[j][i];
+        }
+      }
+      m = mx;
+    }
+  }
+  // Merge the token groups' states.
+  const float M = cross_group_max<LPT>(m);
+  // (l is 0 only where the group saw no token: a NaN score leaves m at -inf too)
+  const float w = l == 0.f ? 0.f : fast_exp2(m - M);
+  const float L = cross_group_sum<LPT>(l * w);
+#pragma unroll
+  for (int j = 0; j < ND; ++j)
+#pragma unroll
+    for (int i = 0; i < VE; ++i) acc[j][i] = cross_group_sum<LPT>(acc[j][i] * w);
+  if (tg != 0) return;
+  if (P.nsplit == 1) {
+    const float inv = 1.f / L;
+#pragma unroll
+    for (int j = 0; j < ND; ++j)
+#pragma unroll
+      for (int i = 0; i < VE; ++i)
+        if (dvalid[j]) out[dim[j] + i] = from_f32<T>(acc[j][i] * inv);
+    return;
+  }
+  const int64_t idx = (row * a.d.q_heads + head) * a.slots + split;
+  if (dg == 0) {
+    a.d.part_ml[idx * 2] = M;
+    a.d.part_ml[idx * 2 + 1] = L;
+  }
+  float* dst = a.d.part_acc + idx * a.d.head_dim;
+#pragma unroll
+  for (int j = 0; j < ND; ++j)
+#pragma unroll
+    for (int i = 0; i < VE; ++i)
+      if (dvalid[j]) dst[dim[j] + i] = acc[j][i];
+}
+
+// One wave per (row, q head): the splits' partials in split order. ND dims a lane.
+template <typename T, int ND>
+__global__ __launch_bounds__(256) void merge_q8_kernel(DecodeQ8Args a) {
+  const int lane = threadIdx.x & 63;
+  const int head = blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int64_t row = a.d.row_base + blockIdx.y;
+  if (head >= a.d.q_heads) return;
+  int64_t trow, qrow;
+  const int n = row_length(row, a.d, &trow, &qrow);
+  if (n <= 0) return;
+  const PartitionQ8 P = partition_q8(n, a);
+  if (P.nsplit <= 1) return;
+  const int64_t idx = (row * a.d.q_heads + head) * a.slots;
+  const float mi = lane < P.nsplit ? a.d.part_ml[(idx + lane) * 2] : -INFINITY;
+  const float li = lane < P.nsplit ? a.d.part_ml[(idx + lane) * 2 + 1] : 0.f;
+  const float M = wave_max(mi);
+  const float wi = lane < P.nsplit ? fast_exp2(mi - M) : 0.f;
+  const float inv = 1.f / wave_sum(wi * li);
+  const float* src = a.d.part_acc + idx * a.d.head_dim;
+  float acc[ND] = {};
+  constexpr int kAhead = 8;
+  for (int s0 = 0; s0 < P.nsplit; s0 += kAhead) {
+    float x[kAhead][ND];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+      for (int j = 0; j < ND; ++j) {
+        const int d = lane + 64 * j;
+        x[u][j] = s0 + u < P.nsplit && d < a.d.head_dim ? src[(int64_t)(s0 + u) * a.d.head_dim + d] : 0.f;
+      }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      if (s0 + u >= P.nsplit) break;
+      const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wi), s0 + u));
+#pragma unroll
+      for (int j = 0; j < ND; ++j) acc[j] = fmaf(w, x[u][j], acc[j]);
+    }
+  }
+  T* out = reinterpret_cast<T*>(a.d.out) + qrow * a.d.o_row + (int64_t)head * a.d.o_head;
+#pragma unroll
+  for (int j = 0; j < ND; ++j)
+    if (lane + 64 * j < a.d.head_dim) out[lane + 64 * j] = from_f32<T>(acc[j] * inv);
+}
+
+template <typename T>
+void launch_valu(bool wide16, bool wide4, dim3 grid, hipStream_t s, const DecodeQ8Args& a) {
+  if (wide16 && a.d.head_dim <= 64)
+    hipLaunchKernelGGL((paged_decode_q8_kernel<T, 16, 4, 1>), grid, dim3(64), 0, s, a);
+  else if (wide16 && a.d.head_dim <= 128)
+    hipLaunchKernelGGL((paged_decode_q8_kernel<T, 16, 8, 1>), grid, dim3(64), 0, s, a);
+  else if (wide16)
+    hipLaunchKernelGGL((paged_decode_q8_kernel<T, 16, 16, 1>), grid, dim3(64), 0, s, a);
+  else if (wide4)
+    hipLaunchKernelGGL((paged_decode_q8_kernel<T, 4, 64, 1>), grid, dim3(64), 0, s, a);
+  else
+    hipLaunchKernelGGL((paged_decode_q8_kernel<T, 1, 64, 4>), grid, dim3(64), 0, s, a);
+}
+
+template <typename T>
+void launch_merge_q8(dim3 grid, hipStream_t s, const DecodeQ8Args& a) {
+  if (a.d.head_dim <= 64) hipLaunchKernelGGL((merge_q8_kernel<T, 1>), grid, dim3(256), 0, s, a);
+  else if (a.d.head_dim <= 128) hipLaunchKernelGGL((merge_q8_kernel<T, 2>), grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((merge_q8_kernel<T, 4>), grid, dim3(256), 0, s, a);
+}
+
+// Pages that a row of this table (and window) can touch, and the splits they make.
+int64_t most_pages(int32_t table_width, int32_t block_size, int32_t window) {
+  const int64_t pages = window > 0 ? std::min<int64_t>(table_width, (int64_t)window / block_size + 2) : table_width;
+  return std::max<int64_t>(1, pages);
+}
+int split_pages(int32_t block_size) { return std::max(1, kSplitTokens / block_size); }
+int most_splits_q8(int32_t table_width, int32_t block_size, int32_t window) {
+  const int64_t pages = most_pages(table_width, block_size, window);
+  return (int)std::min<int64_t>(kMaxSplitsQ8, ceil_div64(pages, split_pages(block_size)));
+}
+
+size_t ml_bytes(int64_t slots) { return ((size_t)slots * 2 * sizeof(float) + 255) & ~(size_t)255; }
+
+}  // namespace
+}  // namespace vrh
+
+using namespace vrh;
+
+extern "C" size_t vrh_paged_decode_q8_workspace_bytes(int64_t rows, int32_t q_heads, int32_t head_dim,
+                                                      int32_t block_size, int32_t table_width,
+                                                      int32_t window) {
+  if (rows <= 0 || q_heads <= 0 || head_dim <= 0 || block_size <= 0 || table_width < 0 || window < 0) return 0;
+  const int splits = most_splits_q8(table_width, block_size, window);
+  if (splits <= 1) return 0;
+  const int64_t slots = rows * q_heads * splits;
+  return ml_bytes(slots) + (size_t)slots * head_dim * sizeof(float);
+}
+
+int vrh_decode_rows_q8(const Q8Call& c, const int32_t* cu_q, int32_t num_seqs, int32_t expand_e,
+                       int64_t rows, int32_t window, void* workspace, size_t workspace_bytes,
+                       bool one_split, hipStream_t s, const char* who) {
+  const int es = dtype_bytes(c.dtype);
+  VRH_CHECK_ARG(es > 0, "%s: unknown dtype %d", who, c.dtype);
+  VRH_CHECK_ARG(rows >= 0 && c.q_heads >= 1 && c.kv_heads >= 1 && c.q_heads % c.kv_heads == 0,
+                "%s: query heads must be a positive multiple of KV heads", who);
+  VRH_CHECK_ARG(c.q_heads <= 65535, "%s: too many heads", who);
+  VRH_CHECK_ARG(c.head_dim >= 1 && c.head_dim <= 256, "%s: head_dim %d unsupported", who, c.head_dim);
+  VRH_CHECK_ARG(c.block_size >= 1 && c.table_width >= 0 && window >= 0 && c.num_blocks >= 1,
+                "%s: bad block_size/table_width/window/num_blocks", who);
+  if (rows == 0) return VRH_OK;
+  VRH_CHECK_ARG(c.out && c.q && c.k && c.v && c.scales && c.lengths && (c.tables || c.table_width == 0),
+                "%s: null pointer", who);
+  DecodeQ8Args a = {};
+  a.scales = (const uint8_t*)c.scales;
+  a.s_block = c.s_block;
+  a.s_head = c.s_head;
+  a.num_blocks = c.num_blocks;
+  a.slots = one_split ? 1 : most_splits_q8(c.table_width, c.block_size, window);
+  const int64_t slots = rows * c.q_heads * a.slots;
+  if (a.slots > 1) {
+    const size_t need = ml_bytes(slots) + (size_t)slots * c.head_dim * sizeof(float);
+    VRH_CHECK_ARG(workspace && workspace_bytes >= need, "%s: workspace of %zu bytes needed, %zu given", who,
+                  need, workspace ? workspace_bytes : (size_t)0);
+    VRH_CHECK_ARG(((uintptr_t)workspace & 255) == 0, "%s: workspace misaligned", who);
+    a.d.part_ml = (float*)workspace;
+    a.d.part_acc = (float*)((char*)workspace + ml_bytes(slots));
+  }
+  a.d.out = c.out;
+  a.d.q = c.q;
+  a.d.k = c.k;
+  a.d.v = c.v;
+  a.d.tables = c.tables;
+  a.d.lengths = c.lengths;
+  a.d.rows = rows;
+  a.d.q_row = c.q_row;
+  a.d.q_head = c.q_head;
+  a.d.o_row = c.o_row;
+  a.d.o_head = c.o_head;
+  a.d.k_block = a.d.v_block = c.c_block;
+  a.d.k_token = a.d.v_token = c.c_token;
+  a.d.k_head = a.d.v_head = c.c_head;
+  a.d.table_stride = c.table_stride;
+  a.d.cu_q = cu_q;
+  a.d.num_seqs = num_seqs;
+  a.d.expand_e = expand_e;
+  a.d.q_heads = c.q_heads;
+  a.d.group = c.q_heads / c.kv_heads;
+  a.d.head_dim = c.head_dim;
+  a.d.block_size = c.block_size;
+  a.d.bs_shift = (c.block_size & (c.block_size - 1)) == 0 ? __builtin_ctz((unsigned)c.block_size) : -1;
+  a.d.window = window;
+  a.d.min_bps = split_pages(c.block_size);
+  a.d.table_width = c.table_width;
+  a.d.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)c.head_dim));
+  auto cache_aligned = [&](int v) {
+    return c.head_dim % v == 0 && c.c_block % v == 0 && c.c_token % v == 0 && c.c_head % v == 0 &&
+           (uintptr_t)c.k % v == 0 && (uintptr_t)c.v % v == 0;
+  };
+  constexpr int64_t kRowsPerLaunch = 65535;
+  for (int64_t first = 0; first < rows; first += kRowsPerLaunch) {
+    a.d.row_base = first;
+    const unsigned count = (unsigned)std::min<int64_t>(rows - first, kRowsPerLaunch);
+    const dim3 grid((unsigned)a.slots, (unsigned)c.q_heads, count);
+    const dim3 mgrid((unsigned)ceil_div(c.q_heads, 4), count);
+    switch (c.dtype) {
+      case VRH_DTYPE_F32:
+        launch_valu<float>(cache_aligned(16), cache_aligned(4), grid, s, a);
+        if (a.slots > 1) launch_merge_q8<float>(mgrid, s, a);
+        break;
+      case VRH_DTYPE_F16:
+        launch_valu<f16_t>(cache_aligned(16), cache_aligned(4), grid, s, a);
+        if (a.slots > 1) launch_merge_q8<f16_t>(mgrid, s, a);
+        break;
+      default:
+        launch_valu<bf16_t>(cache_aligned(16), cache_aligned(4), grid, s, a);
+        if (a.slots > 1) launch_merge_q8<bf16_t>(mgrid, s, a);
+    }
+  }
+  VRH_RETURN_LAUNCH(who);
+}
+
+extern "C" int vrh_paged_decode_q8(int dtype, void* out, const void* q, const void* key_cache,
+                                   const void* value_cache, const void* scales,
+                                   const int32_t* block_tables, const int32_t* context_lengths,
+                                   int64_t rows, int32_t q_heads, int32_t kv_heads, int32_t head_dim,
+                                   int64_t num_blocks, int32_t block_size, int32_t table_width,
+                                   int64_t table_stride, int64_t q_row_stride, int64_t q_head_stride,
+                                   int64_t out_row_stride, int64_t out_head_stride,
+                                   int64_t cache_block_stride, int64_t cache_token_stride,
+                                   int64_t cache_head_stride, int64_t scale_block_stride,
+                                   int64_t scale_head_stride, int32_t window, void* workspace,
+                                   size_t workspace_bytes, vrh_stream_t stream) {
+  const Q8Call c = {dtype, out, q, key_cache, value_cache, scales, block_tables, context_lengths,
+                    q_heads, kv_heads, head_dim, num_blocks, block_size, table_width, table_stride,
+                    q_row_stride, q_head_stride, out_row_stride, out_head_stride, cache_block_stride,
+                    cache_token_stride, cache_head_stride, scale_block_stride, scale_head_stride};
+  return vrh_decode_rows_q8(c, nullptr, 0, 0, rows, window, workspace, workspace_bytes, false,
+                            (hipStream_t)stream, "vrh_paged_decode_q8");
+}

@@ -35,6 +35,7 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "decode_q8.h"
 #include "decode_rows.h"
 
 namespace vrh {
@@ -1132,4 +1133,42 @@ extern "C" int vrh_paged_prefill(int dtype, void* out, const void* q, const void
       launch_prefill_merge<f16_t>(head_dim, tile_blocks, s, a, rows, decode_blocks);
   }
   VRH_RETURN_LAUNCH("vrh_paged_prefill");
+}
+
+// ---------------------------------------------------------------- 8-bit cache
+extern "C" size_t vrh_paged_prefill_q8_workspace_bytes(int64_t num_seqs, int64_t total_q,
+                                                       int32_t max_seqlen_q, int32_t q_heads,
+                                                       int32_t kv_heads, int32_t head_dim,
+                                                       int32_t block_size, int32_t table_width) {
+  return vrh_paged_decode_q8_workspace_bytes(num_seqs * decode_route_q(max_seqlen_q), q_heads, head_dim,
+                                             block_size, table_width, 0);
+}
+
+extern "C" int vrh_paged_prefill_q8(int dtype, void* out, const void* q, const void* key_cache,
+                                    const void* value_cache, const void* scales,
+                                    const int32_t* block_tables, const int32_t* context_lengths,
+                                    const int32_t* cu_seqlens_q, int64_t num_seqs, int64_t total_q,
+                                    int32_t max_seqlen_q, int32_t q_heads, int32_t kv_heads,
+                                    int32_t head_dim, int64_t num_blocks, int32_t block_size,
+                                    int32_t table_width, int64_t table_stride, int64_t q_token_stride,
+                                    int64_t q_head_stride, int64_t out_token_stride,
+                                    int64_t out_head_stride, int64_t cache_block_stride,
+                                    int64_t cache_token_stride, int64_t cache_head_stride,
+                                    int64_t scale_block_stride, int64_t scale_head_stride,
+                                    void* workspace, size_t workspace_bytes, vrh_stream_t stream) {
+  static const char* who = "vrh_paged_prefill_q8";
+  VRH_CHECK_ARG(num_seqs >= 0 && total_q >= 0 && max_seqlen_q >= 0, "%s: bad sizes", who);
+  VRH_CHECK_ARG(num_seqs < (1ll << 31) / kExactQ, "%s: too many sequences", who);
+  if (num_seqs == 0 || total_q == 0) return VRH_OK;
+  VRH_CHECK_ARG(max_seqlen_q >= 1, "%s: max_seqlen_q must be positive", who);
+  VRH_CHECK_ARG(cu_seqlens_q, "%s: null pointer", who);
+  const Q8Call c = {dtype, out, q, key_cache, value_cache, scales, block_tables, context_lengths,
+                    q_heads, kv_heads, head_dim, num_blocks, block_size, table_width, table_stride,
+                    q_token_stride, q_head_stride, out_token_stride, out_head_stride,
+                    cache_block_stride, cache_token_stride, cache_head_stride, scale_block_stride,
+                    scale_head_stride};
+  const bool exact = max_seqlen_q <= kExactQ;
+  return vrh_decode_rows_q8(c, cu_seqlens_q, (int32_t)num_seqs, exact ? max_seqlen_q : 0,
+                            exact ? num_seqs * max_seqlen_q : total_q, 0, workspace, workspace_bytes,
+                            !exact, (hipStream_t)stream, who);
 }

@@ -22,6 +22,8 @@ does on gfx950, given the physical pages the manager resolved:
   copy_blocks     whole-block copy -> vrh_kv_copy_blocks (copy-on-write of a
                   shared page, compaction; no reference counterpart)
 
+``QuantizedKVPool`` is the same pool with 8-bit K and V (no reference counterpart).
+
 Pages are plain block ids. A request's LAST_EXITED layout is one page list
 per loop depth ("plane"); SHARED is one list for every depth. Which pages a
 request owns, and whether a position was written, is the caller's business:
@@ -37,6 +39,7 @@ from numbers import Integral
 import torch
 
 from vllm_rlt.kernels import hip_attention as hip
+from vllm_rlt.kernels import hip_attention_q8 as hip_q8
 
 
 def _count(name: str, value) -> int:
@@ -218,3 +221,85 @@ class PagedKVPool:
             hip.kv_blocks_from_host(self.key_cache, self.value_cache, self._index(pages),
                                     snapshot.keys, snapshot.values)
             torch.cuda.current_stream(self.device).synchronize()
+
+
+class QuantizedKVPool:
+    """K/V pages in 8 bits (e4m3 with a power-of-two scale per block and KV head, see
+    ``kernels/hip_attention_q8``): half the bytes of a 16-bit pool, for queries and new rows in
+    float32, float16 or bfloat16.
+
+    The storage is head-major, ``[num_blocks, num_layers, kv_heads, block_size, head_dim]``, so
+    that what one KV head reads of a block is contiguous (2 KiB at 16 tokens x 128 instead of 16
+    rows of one cache line); ``layer`` gives the usual token-major views of it. Appends take the
+    attention's metadata (block tables, context lengths, cumulative query counts) instead of one
+    address per row: which of a block's tokens are older decides how its scale may change. For
+    LAST_EXITED planes a slot is carried deeper by ``read`` and ``append``, which round it to the
+    target block's scale.
+    """
+
+    def __init__(self, num_blocks, num_layers, block_size, num_kv_heads, head_dim, *,
+                 device="cuda"):
+        self.num_blocks = _count("num_blocks", num_blocks)
+        self.num_layers = _count("num_layers", num_layers)
+        self.block_size = _count("block_size", block_size)
+        self.num_kv_heads = _count("num_kv_heads", num_kv_heads)
+        self.head_dim = _count("head_dim", head_dim)
+        if self.head_dim > 256:
+            raise ValueError("the 8-bit cache supports head_dim <= 256")
+        self.device = torch.device(device)
+        shape = (self.num_blocks, self.num_layers, self.num_kv_heads, self.block_size, self.head_dim)
+        # Zero-filled, so a page that was never written reads as zeros.
+        self.key_store = torch.zeros(shape, dtype=torch.uint8, device=self.device)
+        self.value_store = torch.zeros_like(self.key_store)
+        self.scales = torch.zeros((*shape[:3], 2), dtype=torch.uint8, device=self.device)
+
+    def layer(self, layer: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """One layer's ``[blocks, block_size, kv_heads, head_dim]`` K and V and ``[blocks, kv_heads,
+        2]`` scale exponents."""
+        if isinstance(layer, bool) or not isinstance(layer, Integral) \
+                or not 0 <= layer < self.num_layers:
+            raise ValueError(f"layer must be in [0, {self.num_layers})")
+        return (*(store[:, layer].transpose(1, 2).view(hip_q8.CACHE_DTYPE)
+                  for store in (self.key_store, self.value_store)), self.scales[:, layer])
+
+    def append(self, layer, k, v, block_tables, context_lengths, cu_seqlens_q=None) -> None:
+        """Quantise the newest tokens of every sequence into its pages (``kv_append_q8``)."""
+        hip_q8.kv_append_q8(*self.layer(layer), k, v, block_tables, context_lengths, cu_seqlens_q)
+
+    def attend(self, layer, q, block_tables, context_lengths, *, window=None) -> torch.Tensor:
+        """Single-query paged attention of one layer (``window``: last keys only)."""
+        if window is not None and (type(window) is not int or window <= 0):
+            raise ValueError("window must be a positive integer")
+        return hip_q8.paged_attention_q8(q, *self.layer(layer), block_tables, context_lengths,
+                                         window or 0)
+
+    def prefill(self, layer, q, block_tables, context_lengths, cu_seqlens_q,
+                max_seqlen_q) -> torch.Tensor:
+        """Packed causal prefill of one layer, bottom-right aligned per sequence."""
+        return hip_q8.paged_prefill_attention_q8(q, *self.layer(layer), block_tables,
+                                                 context_lengths, cu_seqlens_q, max_seqlen_q)
+
+    def read(self, layer, pages, length, dtype=torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
+        """The first ``length`` tokens of a page list as ``[length, H, D]`` K and V values."""
+        pages = self._pages("pages", pages)
+        if isinstance(length, bool) or not isinstance(length, Integral) \
+                or not 0 <= length <= len(pages) * self.block_size:
+            raise ValueError("length must be in [0, pages * block_size]")
+        used = self._index(pages[: -(-int(length) // self.block_size)])
+        keys, values = hip_q8.kv_read_q8(*self.layer(layer), used, dtype)
+        return keys.flatten(0, 1)[:length], values.flatten(0, 1)[:length]
+
+    _pages = PagedKVPool._pages
+    _index = PagedKVPool._index
+
+    def copy_blocks(self, src_blocks, dst_blocks) -> None:
+        """``pool[dst[i]] = pool[src[i]]`` for whole blocks: K, V and scales."""
+        src, dst = self._pages("src_blocks", src_blocks), self._pages("dst_blocks", dst_blocks)
+        if len(src) != len(dst):
+            raise ValueError("src_blocks and dst_blocks must have equal lengths")
+        if len(set(dst)) != len(dst) or set(src) & set(dst):
+            raise ValueError("destination blocks must be distinct and disjoint from the sources")
+        if src:
+            index = self._index(src), self._index(dst)
+            hip.kv_copy_blocks(self.key_store, self.value_store, *index)
+            self.scales[index[1]] = self.scales[index[0]]

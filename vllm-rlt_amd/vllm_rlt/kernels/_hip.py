@@ -79,6 +79,35 @@ SIGNATURES: dict[str, tuple[object, list]] = {
     "vrh_gather_segments": (_INT, [_P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P]),
     "vrh_scatter_segments": (_INT, [_P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _P]),
     "vrh_silu_and_mul": (_INT, [_INT, _P, _P, _P, _I64, _P]),
+    "vrh_sequence_metadata": (
+        _INT,
+        [_P, _I64, _I64, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _P, _P, _I64, _I64, _I32, _I32,
+         _I32, _P],
+    ),
+    "vrh_kv_append_q8": (
+        _INT,
+        [_INT, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _P, _I64, _I64, _I64, _I64, _P, _P,
+         _P, _I64, _I64, _I32, _I32, _I64, _I32, _I32, _I64, _P],
+    ),
+    "vrh_kv_read_q8": (
+        _INT,
+        [_INT, _P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _P, _I64, _I32, _I32, _I64, _I32,
+         _P],
+    ),
+    "vrh_paged_decode_q8_workspace_bytes": (_SZ, [_I64, _I32, _I32, _I32, _I32, _I32]),
+    "vrh_paged_decode_q8": (
+        _INT,
+        [_INT, _P, _P, _P, _P, _P, _P, _P, _I64, _I32, _I32, _I32, _I64, _I32, _I32, _I64, _I64,
+         _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I32, _P, _SZ, _P],
+    ),
+    "vrh_paged_prefill_q8_workspace_bytes": (
+        _SZ, [_I64, _I64, _I32, _I32, _I32, _I32, _I32, _I32]
+    ),
+    "vrh_paged_prefill_q8": (
+        _INT,
+        [_INT, _P, _P, _P, _P, _P, _P, _P, _P, _I64, _I64, _I32, _I32, _I32, _I32, _I64, _I32,
+         _I32, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _SZ, _P],
+    ),
 }
 
 

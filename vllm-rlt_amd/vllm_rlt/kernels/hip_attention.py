@@ -578,3 +578,45 @@ def routing_slots(descriptors, slots, n, size):
         lib.vrh_routing_slots(descriptors.data_ptr(), slots.data_ptr(), n, size, _stream(slots)),
         "vrh_routing_slots",
     )
+
+
+def sequence_metadata(tables, table_rows, context_lengths, query_lengths, page, *, tokens,
+                      out_width):
+    """A packed step's metadata from lengths on the GPU, in one launch (``vrh_sequence_metadata``).
+
+    Request r has row ``table_rows[r]`` of ``tables [rows, width]`` and, after the step,
+    ``context_lengths[r]`` tokens whose last ``query_lengths[r]`` are the step's. Returns
+    ``(positions, write_blocks, write_offsets, write_mask, block_tables, context_lengths,
+    cu_seqlens_q)``: the first four per token (``tokens`` of them; those behind the last request
+    are masked and 0), then per request the table padded with -1 to ``out_width``, the length,
+    and the cumulative query counts. Lengths that do not fit the tables or ``tokens`` are cut."""
+    _on_gpu("tables", tables, tables.device)
+    device = tables.device
+    _check_int("tables", tables, torch.int32, 2, device)
+    _check_int("table_rows", table_rows, torch.int64, 1, device)
+    _check_int("context_lengths", context_lengths, torch.int32, 1, device)
+    _check_int("query_lengths", query_lengths, torch.int32, 1, device)
+    n = table_rows.shape[0]
+    if context_lengths.shape[0] != n or query_lengths.shape[0] != n:
+        raise ValueError("table_rows, context_lengths and query_lengths must have equal lengths")
+    if tables.shape[1] > 1 and tables.stride(1) != 1:
+        raise ValueError("tables rows must be contiguous")
+    if page < 1 or tokens < 0 or out_width < 0:
+        raise ValueError("page must be positive, tokens and out_width nonnegative")
+    wide = torch.empty((3, tokens), dtype=torch.int64, device=device)
+    mask = torch.empty(tokens, dtype=torch.bool, device=device)
+    block_tables = torch.empty((n, out_width), dtype=torch.int32, device=device)
+    narrow = torch.empty(2 * n + 1, dtype=torch.int32, device=device)
+    lengths, cu = narrow[:n], narrow[n:]
+    lib = library()
+    lib.check(
+        lib.vrh_sequence_metadata(
+            tables.data_ptr(), tables.shape[0], tables.stride(0), table_rows.contiguous().data_ptr(),
+            context_lengths.contiguous().data_ptr(), query_lengths.contiguous().data_ptr(),
+            wide[0].data_ptr(), wide[1].data_ptr(), wide[2].data_ptr(), mask.data_ptr(),
+            block_tables.data_ptr(), out_width, lengths.data_ptr(), cu.data_ptr(), n, tokens,
+            tables.shape[1], out_width, page, _stream(tables),
+        ),
+        "vrh_sequence_metadata",
+    )
+    return wide[0], wide[1], wide[2], mask, block_tables, lengths, cu

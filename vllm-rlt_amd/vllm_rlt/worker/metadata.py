@@ -128,3 +128,25 @@ def device_kv_metadata(*, position_ids, write_blocks, write_offsets, block_table
         raise ValueError("active_rows must be an int32 scalar on the metadata device")
     return DeviceKVMetadata(position_ids, write_blocks, write_offsets, block_tables,
                             context_lengths, write_mask, active_rows)
+
+
+def sequence_kv_metadata(tables, table_rows, context_lengths, query_lengths, *, block_size, tokens,
+                         width, max_seqlen_q=None) -> DeviceKVMetadata:
+    """``build_kv_metadata`` of a packed step whose lengths live on the GPU: one launch, no host
+    read, so it can be captured into a graph and replayed as requests grow.
+
+    ``tables [rows, pages]`` holds each request's (or request's and depth plane's) page list;
+    request r uses row ``table_rows[r]`` and has, after the step, ``context_lengths[r]`` tokens
+    of which the last ``query_lengths[r]`` are new. ``tokens`` and ``width`` are the step's
+    (bucketed) token count and table width, known on the host; ``max_seqlen_q`` bounds the query
+    lengths (``tokens`` without it). Tokens behind the last request's have ``write_mask`` False."""
+    from vllm_rlt.kernels.hip_attention import sequence_metadata
+
+    if isinstance(block_size, bool) or not isinstance(block_size, int) or block_size <= 0:
+        raise ValueError("block_size must be a positive integer")
+    positions, blocks, offsets, mask, out_tables, lengths, cu = sequence_metadata(
+        tables, table_rows, context_lengths, query_lengths, block_size, tokens=tokens,
+        out_width=width)
+    return DeviceKVMetadata(positions, blocks, offsets, out_tables, lengths, write_mask=mask,
+                            cu_seqlens_q=cu,
+                            max_seqlen_q=max(1, tokens) if max_seqlen_q is None else max_seqlen_q)
