@@ -39,6 +39,8 @@ struct DecodeQ8Args {
   int64_t s_block, s_head;
   int64_t num_blocks;
   int32_t slots;  // most splits of a row
+  int32_t tiles;  // waves of up to 16 q heads per KV head (MFMA kernel)
+  int32_t units;  // kv_heads * tiles
 };
 
 // A page id brought into the pool: an id that is not one of its blocks (a caller's
@@ -71,6 +73,91 @@ __device__ __forceinline__ void q8_values(raw_of<VE> raw, float (&x)[VE]) {
       for (int j = 0; j < 4; ++j) x[i + j] = f[j];
     }
   }
+}
+
+// 16-bit operands of 8 e4m3 bytes, and the products they feed.
+typedef __attribute__((ext_vector_type(8))) __bf16 q8_bf16x8;
+typedef __attribute__((ext_vector_type(8))) _Float16 q8_f16x8;
+typedef __attribute__((ext_vector_type(4))) float q8_f32x4;
+typedef __attribute__((ext_vector_type(16))) float q8_f32x16;
+typedef __attribute__((ext_vector_type(4))) uint32_t q8_u32x4;
+
+template <typename T>
+struct MfmaQ8;
+template <>
+struct MfmaQ8<bf16_t> {
+  // Bytes 0-3 times s0, 4-7 times s1 (powers of two, exact).
+  __device__ static q8_u32x4 widen(uint32_t lo, uint32_t hi, float s0, float s1) {
+    return q8_u32x4{
+        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s0, false)),
+        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, s0, true)),
+        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s1, false)),
+        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, s1, true))};
+  }
+  __device__ static q8_f32x4 run(q8_u32x4 a, q8_u32x4 b, q8_f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(q8_bf16x8, a),
+                                                   __builtin_bit_cast(q8_bf16x8, b), c, 0, 0, 0);
+  }
+};
+template <>
+struct MfmaQ8<f16_t> {
+  __device__ static q8_u32x4 widen(uint32_t lo, uint32_t hi, float s0, float s1) {
+    return q8_u32x4{
+        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, s0, false)),
+        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(lo, s0, true)),
+        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, s1, false)),
+        __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(hi, s1, true))};
+  }
+  __device__ static q8_f32x4 run(q8_u32x4 a, q8_u32x4 b, q8_f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(q8_f16x8, a),
+                                                  __builtin_bit_cast(q8_f16x8, b), c, 0, 0, 0);
+  }
+};
+
+// Softmax weights are rounded to the query's type for the V product: exp2(s - m) where
+// the reference m was the largest score minus kLift when it last moved, and moves when
+// a score passes it by kSlack. bf16 rounds every weight by at most 2^-9 of it. f16 has
+// few exponents: lifted by 2^7 its weights go down to 2^-21 of the largest before they
+// get subnormal (2^-14 unlifted), and up to 2^12 (2^15 with the factor of v_scale).
+template <typename T>
+struct Weights {
+  static constexpr float kLift = 0.f, kSlack = 8.f;
+};
+template <>
+struct Weights<f16_t> {
+  static constexpr float kLift = 7.f, kSlack = 12.f;
+};
+
+// How a page's V scale 2^(e - 127) meets the product: vs in the bytes' conversion, ps
+// on the weights. bf16 holds e4m3 * 2^(e - 127) exactly. f16 does up to 2^7 (448 * 2^7
+// = 57344); what a larger scale has over that goes to the weights. Below 2^-15 the
+// conversion rounds to f16's least step, 2^-24, which the f16 output has as well.
+template <typename T>
+__device__ __forceinline__ void v_scale(int e, float& vs, float& ps) {
+  if constexpr (sizeof(T) == 2 && !__is_same(T, bf16_t)) {
+    vs = q8_scale(min(e, 134));
+    ps = q8_scale(max(e - 134, 0) + 127);
+  } else {
+    vs = q8_scale(e);
+    ps = 1.f;
+  }
+}
+
+// 16 bytes at an LDS byte offset.
+__device__ __forceinline__ q8_u32x4 lds_read16(uint32_t offset) {
+  return *(const q8_u32x4 __attribute__((address_space(3)))*)(uintptr_t)offset;
+}
+
+// s_waitcnt vmcnt(N) for N up to 63, and lgkmcnt(0) (gfx9 encoding).
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  static_assert(N >= 0 && N < 64, "vmcnt");
+  __builtin_amdgcn_s_waitcnt((N & 15) | (N >> 4) << 14 | 0x7 << 4 | 0xF << 8);
+  asm volatile("" ::: "memory");
+}
+__device__ __forceinline__ void wait_lds() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt(15 | 3 << 14 | 0x7 << 4);
 }
 
 }  // namespace vrh

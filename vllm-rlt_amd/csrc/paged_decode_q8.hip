@@ -42,6 +42,19 @@ __device__ __forceinline__ PartitionQ8 partition_q8(int n, const DecodeQ8Args& a
   return p;
 }
 
+__device__ __forceinline__ int page_of(int pos, const DecodeQ8Args& a) {
+  return a.d.bs_shift >= 0 ? pos >> a.d.bs_shift : pos / a.d.block_size;
+}
+
+// The (row, split) of a workgroup: item blockIdx.x / units, split-major within a row,
+// rows in order.
+__device__ __forceinline__ bool q8_item(const DecodeQ8Args& a, int64_t& row, int& split) {
+  const int64_t item = blockIdx.x / a.units;
+  row = a.d.row_base + item / a.slots;
+  split = (int)(item - (item / a.slots) * a.slots);
+  return true;
+}
+
 // ------------------------------------------------------ any shape, VALU
 // One wave per (split, q head, row). LPT lanes cover a token's head_dim with VE
 // elements each (ND vectors of VE, LPT * VE apart, where that is not enough), so a
@@ -202,6 +215,302 @@ __global__ __launch_bounds__(64) void paged_decode_q8_kernel(DecodeQ8Args a) {
       if (dvalid[j]) dst[dim[j] + i] = acc[j][i];
 }
 
+// ------------------------------------------------ 16-bit queries on MFMA
+// One wave per (split, KV head, row) serves up to 16 q heads of the KV head (the
+// columns of v_mfma_f32_16x16x32; groups of more take several waves):
+//  * K and V come in chunks of 32 tokens straight into a ring of kStages wave-private
+//    LDS stages, kStages - 1 chunks ahead: no registers are held by loads in flight and
+//    no barrier is needed. One load instruction covers RPI whole rows of one page.
+//  * S^T = K Q^T per 16 tokens: bytes are converted to the query's type (exact), 16 a
+//    lane per LDS read, which is two k-steps; the dims of Q^T's k-slots follow that
+//    order. The page's K scale joins the softmax scale on the fp32 scores.
+//  * O^T += V^T P^T per 32 tokens: the S accumulators, rounded to the query's type, are
+//    the P^T operand; one ds_read_b64_tr_b8 returns 8 tokens of a dim for V^T, whose
+//    conversion applies the page's scale (exact in bf16; in f16 see v_scale).
+//  * A row of LDS is D bytes of 16-byte chunks, chunk c of row r stored at slot
+//    c ^ swizzle(r), so that both readers spread over all banks.
+constexpr int kChunk = 32;  // tokens per stage
+constexpr int kStages = 3;
+
+typedef __attribute__((ext_vector_type(4))) float f32x4_t;
+typedef __attribute__((ext_vector_type(4))) uint32_t u32x4_t;
+typedef __attribute__((ext_vector_type(2))) uint32_t u32x2_t;
+
+// ds_read_b64_tr_b8: within each 16-lane group lane j receives byte j % 8 of the 8-byte
+// chunks addressed by lanes 2i + j / 8, i = 0..7 (byte i of the result): lanes 2i, 2i + 1
+// that address 16 bytes of row i give lane j column j of rows 0..7.
+__device__ __forceinline__ u32x2_t lds_tr8(uint32_t offset) {
+  typedef int v2i __attribute__((ext_vector_type(2)));
+  const v2i r = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+      (v2i __attribute__((address_space(3)))*)(uintptr_t)offset);
+  return __builtin_bit_cast(u32x2_t, r);
+}
+
+template <int D>
+__device__ __forceinline__ int q8_swizzle(int row) {
+  if constexpr (D == 128) {
+    const int i = row >> 1;
+    return (i & 3) | (((i >> 2) ^ (i >> 3)) & 1) << 2;
+  } else {
+    const int i = row >> 2;
+    return (i & 1) | (((i >> 1) ^ (i >> 2)) & 1) << 1;
+  }
+}
+
+// global_load_lds_dword: 4 bytes per lane to m0 + 4 * lane (see lds_dma16).
+__device__ __forceinline__ void lds_dma4(const void* g, uint32_t m0) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(g), "{m0}"(m0) : "memory");
+}
+
+template <typename T, int D>
+__global__ __launch_bounds__(64) void paged_decode_q8_mfma_kernel(DecodeQ8Args a) {
+  constexpr int KCH = D / 16;        // 16-byte chunks per row
+  constexpr int RPI = 64 / KCH;      // rows per load instruction
+  constexpr int NI = kChunk / RPI;   // load instructions per chunk, K and V each
+  constexpr int KC = D / 64;         // LDS reads per 16 tokens of K
+  constexpr int DT = D / 16;         // 16-dim tiles of O^T
+  constexpr int kStage = 2 * kChunk * D;
+  __shared__ __attribute__((aligned(256))) uint8_t stage[kStages * kStage + 256];
+  const int lane = threadIdx.x;
+  const int col = lane & 15, grp = lane >> 4;
+
+  int64_t row;
+  int split;
+  if (!q8_item(a, row, split)) return;
+  const int unit = (int)(blockIdx.x % a.units);
+  const int kvh = unit / a.tiles;
+  const int head0 = kvh * a.d.group + (unit - kvh * a.tiles) * 16;
+  const int heads = min(16, (kvh + 1) * a.d.group - head0);
+  int64_t trow, qrow;
+  const int n = row_length(row, a.d, &trow, &qrow);
+  if (n < 0) return;
+  const bool hcol = col < heads;
+  T* out = reinterpret_cast<T*>(a.d.out) + qrow * a.d.o_row + (int64_t)(head0 + col) * a.d.o_head + 4 * grp;
+  if (n == 0) {
+    if (split == 0 && hcol) {
+#pragma unroll
+      for (int t = 0; t < DT; ++t) *reinterpret_cast<u32x2_t*>(out + 16 * t) = u32x2_t{0u, 0u};
+    }
+    return;
+  }
+  const PartitionQ8 P = partition_q8(n, a);
+  if (split >= P.nsplit) return;
+  const int bs = a.d.block_size;
+  const int s0 = P.first + split * P.bps, s1 = min(s0 + P.bps, P.first + P.pages);
+  const int32_t* table = a.d.tables + trow * a.d.table_stride;
+
+  // Q^T operands of k-step (c, i): dims 64 c + 16 grp + 8 i .. + 7.
+  u32x4_t qop[KC][2];
+  {
+    const T* qp = reinterpret_cast<const T*>(a.d.q) + qrow * a.d.q_row +
+                  (int64_t)(head0 + (hcol ? col : 0)) * a.d.q_head + 16 * grp;
+#pragma unroll
+    for (int c = 0; c < KC; ++c)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const u32x4_t x = *reinterpret_cast<const u32x4_t*>(qp + 64 * c + 8 * i);
+        qop[c][i] = hcol ? x : u32x4_t{0u, 0u, 0u, 0u};
+      }
+  }
+  const uint8_t* kbase = reinterpret_cast<const uint8_t*>(a.d.k) + (int64_t)kvh * a.d.k_head;
+  const uint8_t* vbase = reinterpret_cast<const uint8_t*>(a.d.v) + (int64_t)kvh * a.d.v_head;
+  const uint8_t* sbase = a.scales + (int64_t)kvh * a.s_head;
+  const uint32_t lds0 = lds_offset(stage);
+  const uint32_t lds_sc = lds0 + kStages * kStage;
+
+  // This lane's byte offset within a load instruction's rows; instructions whose rows
+  // have the swizzle's top bit flipped take the second.
+  const int lrow = lane / KCH;
+  uint32_t loff[2];
+#pragma unroll
+  for (int x = 0; x < 2; ++x)
+    loff[x] = (uint32_t)lrow * (uint32_t)a.d.k_token +
+              16 * ((lane % KCH) ^ q8_swizzle<D>(lrow) ^ (x * KCH / 2));
+  auto flip = [](int r) { return D == 128 ? (r ^ (r >> 1)) & 1 : r & 1; };
+  // LDS byte offsets of the operand reads.
+  uint32_t koff[2];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) koff[t] = lds0 + (16 * t + col) * D + 16 * (grp ^ q8_swizzle<D>(16 * t + col));
+  const int vrow = (col >> 1) < 4 ? 4 * grp + (col >> 1) : 12 + 4 * grp + (col >> 1);
+  const uint32_t voff = lds0 + kChunk * D + vrow * D + 16 * q8_swizzle<D>(vrow) + 8 * (col & 1);
+
+  float m = -1e30f, lsum = 0.f;  // of this lane's head column; lsum over its token slots
+  f32x4_t acc[DT];
+#pragma unroll
+  for (int t = 0; t < DT; ++t) acc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+
+  for (int seg = s0; seg < s1; seg += 64) {
+    const int seg1 = min(s1, seg + 64);
+    const int blk = seg + lane < seg1 ? pool_block(table[seg + lane], a) : 0;
+    // The pages' exponents: the aligned word around each pair, and which half it is.
+    const uint8_t* sp = sbase + (int64_t)blk * a.s_block;
+    const uint64_t high = __ballot(((uintptr_t)sp & 2) != 0);
+    lds_dma4((const void*)((uintptr_t)sp & ~(uintptr_t)3), __builtin_amdgcn_readfirstlane(lds_sc));
+    const int t0 = seg * bs;  // first token of the segment
+    const int tb = max(P.start, t0);
+    const int te = (int)min((int64_t)n, (int64_t)seg1 * bs);
+    // Chunks start at the 16-token step of the page that the first token is in.
+    const int c0 = t0 + ((tb - t0) & ~15);
+    const int chunks = (te - c0 + kChunk - 1) / kChunk;
+
+    auto load = [&](int j, auto st_c) {
+      constexpr int st = decltype(st_c)::value;
+      const int p0 = c0 + j * kChunk;
+      const uint32_t kl = lds0 + st * kStage, vl = kl + kChunk * D;
+      if (p0 >= tb && te - p0 >= kChunk) {
+        int page = (int)__builtin_amdgcn_readfirstlane(page_of(p0, a) - seg);
+        int off = p0 - (seg + page) * bs;
+#pragma unroll
+        for (int r = 0; r < NI; ++r) {
+          const uint32_t b = __builtin_amdgcn_readlane(blk, page);
+          const uint64_t at = (uint64_t)b * (uint64_t)a.d.k_block + (uint64_t)((uint32_t)off * (uint64_t)(uint32_t)a.d.k_token);
+          lds_dma16_s(kbase + at, loff[flip(r)], __builtin_amdgcn_readfirstlane(kl + 1024 * r));
+          lds_dma16_s(vbase + at, loff[flip(r)], __builtin_amdgcn_readfirstlane(vl + 1024 * r));
+          off += RPI;
+          if (off >= bs) {
+            off -= bs;
+            ++page;
+          }
+        }
+        return;
+      }
+      // A chunk that reaches outside the visible tokens reads the nearest visible one
+      // there: masked out of the softmax, and as finite as the row itself.
+#pragma unroll
+      for (int r = 0; r < NI; ++r) {
+        const int i = RPI * r + lrow;
+        const int pos = max(tb, te - p0 > i ? p0 + i : te - 1);
+        const int page = page_of(pos, a) - seg;
+        const int off = pos - (seg + page) * bs;
+        const int64_t at = (int64_t)shfl_i32(blk, page) * a.d.k_block + (int64_t)off * a.d.k_token +
+                           16 * ((lane % KCH) ^ q8_swizzle<D>(i));
+        lds_dma16(kbase + at, __builtin_amdgcn_readfirstlane(kl + 1024 * r));
+        lds_dma16(vbase + at, __builtin_amdgcn_readfirstlane(vl + 1024 * r));
+      }
+    };
+    auto attend = [&](int j, auto st_c) {
+      constexpr int st = decltype(st_c)::value;
+      const int p0 = c0 + j * kChunk;
+      // Scales of the chunk's two 16-token tiles.
+      float ks[2], vs[2], ps[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int pos = min(max(p0 + 16 * t, tb), te - 1);
+        const int page = __builtin_amdgcn_readfirstlane(page_of(pos, a) - seg);
+        const uint32_t w = __builtin_amdgcn_readfirstlane(
+            *reinterpret_cast<const uint32_t*>(stage + kStages * kStage + 4 * page));
+        const uint32_t e = w >> ((high >> page & 1) ? 16 : 0);
+        ks[t] = q8_scale(e & 255) * a.d.scale_log2;
+        v_scale<T>(e >> 8 & 255, vs[t], ps[t]);
+      }
+      f32x4_t sc[2];
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        sc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+          const u32x4_t x = lds_read16((koff[t] ^ (64 * c)) + st * kStage);
+          sc[t] = MfmaQ8<T>::run(MfmaQ8<T>::widen(x[0], x[1], 1.f, 1.f), qop[c][0], sc[t]);
+          sc[t] = MfmaQ8<T>::run(MfmaQ8<T>::widen(x[2], x[3], 1.f, 1.f), qop[c][1], sc[t]);
+        }
+      }
+      float mx = -INFINITY;
+      if (p0 >= tb && te - p0 >= kChunk) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            sc[t][i] *= ks[t];
+            mx = fmaxf(mx, sc[t][i]);
+          }
+      } else {
+        const int lo = tb - p0 - 4 * grp, hi = te - p0 - 4 * grp;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            sc[t][i] = 16 * t + i >= lo && 16 * t + i < hi ? sc[t][i] * ks[t] : -INFINITY;
+            mx = fmaxf(mx, sc[t][i]);
+          }
+      }
+      // Over the four lane groups of the head column.
+      {
+        const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+        mx = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+        const auto y = __builtin_amdgcn_permlane16_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+        mx = fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
+      }
+      // The reference moves only when a score passes it by more than kSlack, so that most
+      // chunks leave the accumulators alone.
+      if (__any(mx > m + Weights<T>::kSlack)) {
+        const float top = fmaxf(m, mx - Weights<T>::kLift);
+        const float corr = fast_exp2(m - top);
+        lsum *= corr;
+#pragma unroll
+        for (int t = 0; t < DT; ++t) acc[t] *= corr;
+        m = top;
+      }
+      float p[2][4];
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          p[t][i] = fast_exp2(sc[t][i] - m);
+          lsum += p[t][i];
+          if constexpr (std::is_same<T, f16_t>::value) p[t][i] *= ps[t];
+        }
+      const u32x4_t pop = u32x4_t{pack2<T>(p[0][0], p[0][1]), pack2<T>(p[0][2], p[0][3]),
+                                  pack2<T>(p[1][0], p[1][1]), pack2<T>(p[1][2], p[1][3])};
+#pragma unroll
+      for (int t = 0; t < DT; ++t) {
+        const u32x2_t x = lds_tr8((voff ^ (16 * t)) + st * kStage);
+        acc[t] = MfmaQ8<T>::run(MfmaQ8<T>::widen(x[0], x[1], vs[0], vs[1]), pop, acc[t]);
+      }
+    };
+    using S0 = std::integral_constant<int, 0>;
+    using S1 = std::integral_constant<int, 1>;
+    using S2 = std::integral_constant<int, 2>;
+    static_assert(kStages == 3, "the steps below");
+    load(0, S0{});
+    if (chunks > 1) load(1, S1{});
+    // Step j: chunk j has landed (only the loads of j + 1 may be in flight); the stage of
+    // j - 1, whose reads have returned, takes chunk j + 2.
+    auto step = [&](int j, auto now, auto next) {
+      if (j + 1 < chunks) wait_loads<2 * NI>();
+      else wait_loads<0>();
+      if (j + 2 < chunks) load(j + 2, next);
+      attend(j, now);
+      wait_lds();
+    };
+    for (int j = 0; j < chunks; j += 3) {
+      step(j, S0{}, S2{});
+      if (j + 1 >= chunks) break;
+      step(j + 1, S1{}, S0{});
+      if (j + 2 >= chunks) break;
+      step(j + 2, S2{}, S1{});
+    }
+  }
+  lsum += shfl_xor_f32(lsum, 16);
+  lsum += shfl_xor_f32(lsum, 32);
+  if (!hcol) return;
+  if (P.nsplit == 1) {
+    const float inv = 1.f / lsum;
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+      *reinterpret_cast<u32x2_t*>(out + 16 * t) =
+          u32x2_t{pack2<T>(acc[t][0] * inv, acc[t][1] * inv), pack2<T>(acc[t][2] * inv, acc[t][3] * inv)};
+    return;
+  }
+  const int64_t idx = (row * a.d.q_heads + head0 + col) * a.slots + split;
+  if (grp == 0) {
+    a.d.part_ml[idx * 2] = m;
+    a.d.part_ml[idx * 2 + 1] = lsum;
+  }
+  float* dst = a.d.part_acc + idx * D + 4 * grp;
+#pragma unroll
+  for (int t = 0; t < DT; ++t) *reinterpret_cast<f32x4_t*>(dst + 16 * t) = acc[t];
+}
+
 // One wave per (row, q head): the splits' partials in split order. ND dims a lane.
 template <typename T, int ND>
 __global__ __launch_bounds__(256) void merge_q8_kernel(DecodeQ8Args a) {
@@ -265,6 +574,14 @@ void launch_merge_q8(dim3 grid, hipStream_t s, const DecodeQ8Args& a) {
   if (a.d.head_dim <= 64) hipLaunchKernelGGL((merge_q8_kernel<T, 1>), grid, dim3(256), 0, s, a);
   else if (a.d.head_dim <= 128) hipLaunchKernelGGL((merge_q8_kernel<T, 2>), grid, dim3(256), 0, s, a);
   else hipLaunchKernelGGL((merge_q8_kernel<T, 4>), grid, dim3(256), 0, s, a);
+}
+
+template <typename T>
+void launch_mfma_q8(unsigned groups, hipStream_t s, const DecodeQ8Args& a) {
+  if (a.d.head_dim == 128)
+    hipLaunchKernelGGL((paged_decode_q8_mfma_kernel<T, 128>), dim3(groups), dim3(64), 0, s, a);
+  else
+    hipLaunchKernelGGL((paged_decode_q8_mfma_kernel<T, 64>), dim3(groups), dim3(64), 0, s, a);
 }
 
 // Pages that a row of this table (and window) can touch, and the splits they make.
@@ -355,7 +672,20 @@ int vrh_decode_rows_q8(const Q8Call& c, const int32_t* cu_q, int32_t num_seqs, i
     return c.head_dim % v == 0 && c.c_block % v == 0 && c.c_token % v == 0 && c.c_head % v == 0 &&
            (uintptr_t)c.k % v == 0 && (uintptr_t)c.v % v == 0;
   };
-  constexpr int64_t kRowsPerLaunch = 65535;
+  // The matrix kernel: 16-bit queries, head_dim 64 or 128, whole 16-token steps of a
+  // page, 16-byte aligned rows, scale pairs that do not straddle a word, row offsets
+  // within a load instruction in 32 bits.
+  const bool mfma = c.dtype != VRH_DTYPE_F32 && (c.head_dim == 64 || c.head_dim == 128) &&
+                    c.block_size % 16 == 0 && c.block_size <= 65536 && cache_aligned(16) && c.c_token < (1 << 26) &&
+                    c.c_token >= 0 && c.c_block >= 0 && c.q_row % 8 == 0 && c.q_head % 8 == 0 &&
+                    c.o_row % 4 == 0 && c.o_head % 4 == 0 && (uintptr_t)c.q % 16 == 0 &&
+                    (uintptr_t)c.out % 8 == 0 && c.s_block % 2 == 0 && c.s_head % 2 == 0 &&
+                    (uintptr_t)c.scales % 2 == 0;
+  a.tiles = ceil_div(a.d.group, 16);
+  a.units = c.kv_heads * a.tiles;
+  const int64_t per_row = mfma ? (int64_t)a.units * a.slots : 1;
+  VRH_CHECK_ARG(per_row < (1ll << 30), "%s: too many heads", who);
+  const int64_t kRowsPerLaunch = std::min<int64_t>(65535, (1ll << 31) / per_row - 1);
   for (int64_t first = 0; first < rows; first += kRowsPerLaunch) {
     a.d.row_base = first;
     const unsigned count = (unsigned)std::min<int64_t>(rows - first, kRowsPerLaunch);
@@ -367,11 +697,13 @@ int vrh_decode_rows_q8(const Q8Call& c, const int32_t* cu_q, int32_t num_seqs, i
         if (a.slots > 1) launch_merge_q8<float>(mgrid, s, a);
         break;
       case VRH_DTYPE_F16:
-        launch_valu<f16_t>(cache_aligned(16), cache_aligned(4), grid, s, a);
+        if (mfma) launch_mfma_q8<f16_t>((unsigned)(count * per_row), s, a);
+        else launch_valu<f16_t>(cache_aligned(16), cache_aligned(4), grid, s, a);
         if (a.slots > 1) launch_merge_q8<f16_t>(mgrid, s, a);
         break;
       default:
-        launch_valu<bf16_t>(cache_aligned(16), cache_aligned(4), grid, s, a);
+        if (mfma) launch_mfma_q8<bf16_t>((unsigned)(count * per_row), s, a);
+        else launch_valu<bf16_t>(cache_aligned(16), cache_aligned(4), grid, s, a);
         if (a.slots > 1) launch_merge_q8<bf16_t>(mgrid, s, a);
     }
   }
