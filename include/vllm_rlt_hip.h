@@ -410,7 +410,7 @@ int vrh_paged_decode_q8(int dtype, void* out, const void* q, const void* key_cac
  * cu_seqlens_q[num_seqs]) belong to no sequence and their output is left. With
  * max_seqlen_q <= 8 every query equals, bit for bit, vrh_paged_decode_q8 of a row with
  * its length. */
-size_t vrh_paged_prefill_q8_workspace_bytes(int64_t num_seqs, int64_t total_q,
+size_t vrh_paged_prefill_q8_workspace_bytes(int dtype, int64_t num_seqs, int64_t total_q,
                                             int32_t max_seqlen_q, int32_t q_heads,
                                             int32_t kv_heads, int32_t head_dim,
                                             int32_t block_size, int32_t table_width);

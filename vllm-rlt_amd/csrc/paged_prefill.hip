@@ -116,6 +116,15 @@ struct PrefillArgs {
   int32_t rank_in_kernel; // num_seqs <= 64: each wave ranks the sequences itself
   int32_t compact;        // grid over the numbered tiles (rank_in_kernel, kv_heads % 8 == 0)
   float scale_log2;
+  // 8-bit cache (k, v in bytes): scale exponents and the pool's blocks.
+  const uint8_t* scales;
+  int64_t s_block, s_head;
+  int64_t num_blocks;
+};
+
+// Type tag of the 8-bit cache (a 16-bit cache has the query's type).
+struct e4m3_t {
+  uint8_t bits;
 };
 
 // LDS tiles (one 32-key sub-block of K and of V per stage), both row-major
@@ -144,6 +153,32 @@ struct Lds {
   }
 };
 
+// The same for the 8-bit cache: rows of D bytes, chunk c of row r at slot c ^ swizzle(r).
+// Both readers are conflict free at D = 64 and 128: the K operand read (16 rows, one
+// chunk each, per quarter wave) and the transposed V read (rows 0-3 and 8-11, or 4-7 and
+// 12-15, of two neighbouring chunks per half wave).
+template <int D>
+struct Lds8 {
+  static constexpr int KCH = D / 16;
+  static constexpr bool kPow2 = (KCH & (KCH - 1)) == 0;
+  __device__ static int swizzle(int row) {
+    if constexpr (KCH == 8) {
+      const int i = row >> 1;
+      return (i & 4) | (i & 1) << 1 | (i >> 1 & 1);
+    } else if constexpr (KCH == 4) {
+      return row >> 2 & 3;
+    } else if constexpr (KCH == 2) {
+      return row >> 3 & 1;
+    } else {
+      return 0;  // KCH = 6: no XOR stays inside the row
+    }
+  }
+  // Byte offset `base` of chunk 0 or 1 of a row moved by 2 c chunks.
+  __device__ static uint32_t chunk(uint32_t base, int c) {
+    return kPow2 ? base ^ (32u * c) : base + 32u * c;
+  }
+};
+
 // ds_read_b64_tr_b16: within each 16-lane group, lane j receives element j % 4
 // of the 8-byte chunks addressed by lanes 4i + j / 4, i = 0..3 (element i of
 // the result). Lanes 4i + s that address row (key) r0 + i, dims d0 + 4s .. +3
@@ -153,6 +188,21 @@ __device__ __forceinline__ u32x2 lds_read_tr16(const uint16_t* p) {
   const v4s r = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
       (v4s __attribute__((address_space(3)))*)(const_cast<uint16_t*>(p)));
   return __builtin_bit_cast(u32x2, r);
+}
+
+// ds_read_b64_tr_b8: lane j of a 16-lane group receives byte j % 8 of the 8-byte chunks
+// addressed by lanes 2i + j / 8, i = 0..7 (byte i of the result): lanes 2i, 2i + 1 that
+// address 16 bytes of row i give lane j column j of the 8 rows.
+__device__ __forceinline__ u32x2 lds_read_tr8(const char* p) {
+  typedef int v2i __attribute__((ext_vector_type(2)));
+  const v2i r = __builtin_amdgcn_ds_read_tr8_b64_v2i32(
+      (v2i __attribute__((address_space(3)))*)(const_cast<char*>(p)));
+  return __builtin_bit_cast(u32x2, r);
+}
+
+// 1 in each byte that is an e4m3 NaN (0x7F or 0xFF), 0 in the others.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t x) {
+  return (((x & 0x7F7F7F7Fu) + 0x01010101u) >> 7) & 0x01010101u;
 }
 
 // Three workgroups per CU, three waves per SIMD.
@@ -221,19 +271,25 @@ __device__ __forceinline__ int split_run(const Batch& b, const PrefillArgs& a) {
 // Page addressing modes: kDiv (any block size), kShift (power of two).
 enum PageMode { kDiv = 0, kShift = 1 };
 
-template <typename T, int D, int MODE>
+// T: type of q and out; C: of the cache (T, or e4m3_t with a power-of-two scale per page
+// and KV head: bytes are staged as they are and widened to T on their way from LDS into
+// the MFMA operands, K unscaled (its scale joins the softmax scale on the scores), V with
+// its scale).
+template <typename T, typename C, int D, int MODE>
 __global__ __launch_bounds__(kThreads, kWgPerCu)
 __attribute__((amdgpu_waves_per_eu(kWavesPerEu, kWavesPerEu))) void paged_prefill_kernel(PrefillArgs a) {
   constexpr int DC = D / 16;                   // 16-wide d chunks (QK^T k-steps)
   constexpr int DB = D / 32;                   // 32-row d blocks of O^T
-  constexpr int KCH = D / 8;                   // 16-byte chunks per key row
+  constexpr bool kQ8 = sizeof(C) == 1;
+  constexpr int KCH = D * (int)sizeof(C) / 16; // 16-byte chunks per key row
+  constexpr int CPE = 16 / (int)sizeof(C);     // elements per chunk
   constexpr int SB_INST = kSB * KCH / 64;      // 16-byte wave stores per sub-block (K or V)
   constexpr int NI = (SB_INST + kWaves - 1) / kWaves;  // per wave (the last may be idle)
   static_assert(D % 32 == 0 && D <= 128, "head_dim");
-  using L = Lds<D>;
+  using L = std::conditional_t<kQ8, Lds8<D>, Lds<D>>;
 
-  __shared__ __attribute__((aligned(16))) uint16_t ks[kStages][L::kElems];
-  __shared__ __attribute__((aligned(16))) uint16_t vs[kStages][L::kElems];
+  __shared__ __attribute__((aligned(kQ8 ? 256 : 16))) C ks[kStages][kSB * D];
+  __shared__ __attribute__((aligned(kQ8 ? 256 : 16))) C vs[kStages][kSB * D];
 
   const int tid = threadIdx.x;
   const int lane = tid & 63;
@@ -321,14 +377,16 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerEu, kWavesPerEu))) void paged_prefil
                          : (max(0, min(end, prefix + (v0 + kWQ - 1) / a.group + 1)) + kSB - 1) / kSB;
   const int32_t* table = a.tables + seq * a.table_stride;
 
-  // Q^T B-operands: lane holds query `col`, dims 16c + 8*half .. +8.
+  // Q^T B-operands: lane holds query `col`, dims 16c + 8*half .. +8 (8-bit cache: k-steps
+  // 2c and 2c + 1 are the halves of one 16-byte K read, dims 32c + 16*half .. +16).
   u32x4 qop[DC];
   {
     const T* qp = reinterpret_cast<const T*>(a.q) + (int64_t)(q_begin + (q_ok ? qi : 0)) * a.q_token +
-                  head * a.q_head + 8 * half;
+                  head * a.q_head + (kQ8 ? 16 : 8) * half;
 #pragma unroll
     for (int c = 0; c < DC; ++c) {
-      const u32x4 v = *reinterpret_cast<const u32x4*>(qp + 16 * c);
+      const u32x4 v =
+          *reinterpret_cast<const u32x4*>(qp + (kQ8 ? 32 * (c >> 1) + 8 * (c & 1) : 16 * c));
       qop[c] = q_ok ? v : u32x4{0, 0, 0, 0};
     }
   }
@@ -341,8 +399,8 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerEu, kWavesPerEu))) void paged_prefil
   float m = -1e30f;
   float lsum = 0.f;     // partial sum over this lane's key slots
 
-  const T* kg = reinterpret_cast<const T*>(a.k) + kvh * a.k_head;
-  const T* vg = reinterpret_cast<const T*>(a.v) + kvh * a.v_head;
+  const C* kg = reinterpret_cast<const C*>(a.k) + kvh * a.k_head;
+  const C* vg = reinterpret_cast<const C*>(a.v) + kvh * a.v_head;
 
   // A 512-entry segment of the page table is staged in LDS. A page id
   // fetched with a vector load would make every later K/V load wait for all
@@ -350,17 +408,30 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerEu, kWavesPerEu))) void paged_prefil
   // the segment is refilled (all waves, between barriers) when a sub-block's
   // pages run past it.
   __shared__ int32_t tbl_lds[kTableSeg];
+  __shared__ uint16_t scale_lds[kQ8 ? kTableSeg : 1];  // the pages' exponents (K, V << 8)
   int tbl_base = 0;
-  auto load_table = [&](int base) {
-    __syncthreads();
-    for (int i = tid; i < kTableSeg; i += kThreads)
-      tbl_lds[i] = base + i < a.table_width ? table[base + i] : 0;
-    __syncthreads();
-    tbl_base = base;
-  };
   auto page_of = [&](int pos) {
     if constexpr (MODE == kDiv) return pos / a.block_size;
     else return pos >> a.bs_shift;
+  };
+  auto load_table = [&](int base) {
+    __syncthreads();
+    for (int i = tid; i < kTableSeg; i += kThreads) {
+      if constexpr (kQ8) {
+        int id = 0;
+        uint32_t e = 0;
+        if (end > 0 && base + i <= page_of(end - 1)) {
+          id = (int)max((int64_t)0, min((int64_t)table[base + i], a.num_blocks - 1));
+          e = q8_exponents(a.scales + (int64_t)id * a.s_block + kvh * a.s_head);
+        }
+        tbl_lds[i] = id;
+        scale_lds[i] = (uint16_t)e;
+      } else {
+        tbl_lds[i] = base + i < a.table_width ? table[base + i] : 0;
+      }
+    }
+    __syncthreads();
+    tbl_base = base;
   };
   load_table(page_of(j0 * kSB));
 
@@ -381,16 +452,16 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerEu, kWavesPerEu))) void paged_prefil
   constexpr int IR = 64 / KCH;
   static_assert(!kPow2 || S % 16 == 0, "swizzle period");
   const int lane_row = (64 * wave + lane) / KCH;
-  const int lane_dof = kPow2 ? (((64 * wave + lane) % KCH) ^ L::swizzle(lane_row)) * 8 : 0;
+  const int lane_dof = kPow2 ? (((64 * wave + lane) % KCH) ^ L::swizzle(lane_row)) * CPE : 0;
   const int lane_in = lane / KCH;  // row within one instruction's IR rows
-  const T* lane_k = kg + (int64_t)lane_row * a.k_token + lane_dof;
-  const T* lane_v = vg + (int64_t)lane_row * a.v_token + lane_dof;
-  const T* lane_k1 = kg + (int64_t)lane_in * a.k_token + lane_dof;
-  const T* lane_v1 = vg + (int64_t)lane_in * a.v_token + lane_dof;
+  const C* lane_k = kg + (int64_t)lane_row * a.k_token + lane_dof;
+  const C* lane_v = vg + (int64_t)lane_row * a.v_token + lane_dof;
+  const C* lane_k1 = kg + (int64_t)lane_in * a.k_token + lane_dof;
+  const C* lane_v1 = vg + (int64_t)lane_in * a.v_token + lane_dof;
   // Byte offset of this lane's 16 bytes within one staging instruction's rows
   // (same for K and V when their strides match); 32-bit when it fits.
-  const int64_t lane_koff64 = ((int64_t)lane_in * a.k_token + lane_dof) * (int64_t)sizeof(T);
-  const bool lane_off32 = (int64_t)(IR - 1) * a.k_token * (int64_t)sizeof(T) + 2 * D < (1ll << 31);
+  const int64_t lane_koff64 = ((int64_t)lane_in * a.k_token + lane_dof) * (int64_t)sizeof(C);
+  const bool lane_off32 = (int64_t)(IR - 1) * a.k_token * (int64_t)sizeof(C) + 2 * D < (1ll << 31);
   const uint32_t lane_koff = (uint32_t)lane_koff64;
   // Addresses of sub-block j's K and V vectors for this wave's staging
   // instructions r = 0 .. NI - 1, handed to `sink(r, k_ptr, v_ptr)`.
@@ -437,7 +508,7 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerEu, kWavesPerEu))) void paged_prefil
       if (pad(inst)) continue;
       const int v = 64 * inst + lane;
       const int row = kPow2 ? lane_row + r * S : v / KCH;
-      const int dof = kPow2 ? 0 : ((v % KCH) ^ L::swizzle(row)) * 8;
+      const int dof = kPow2 ? 0 : ((v % KCH) ^ L::swizzle(row)) * CPE;
       const int pos = min(k0 + row, end - 1);
       const int pg = page_of(pos);
       const int64_t page = tbl_lds[pg - tbl_base];
@@ -483,11 +554,11 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerEu, kWavesPerEu))) void paged_prefil
       }
       return;
     }
-    const T* kp[NI];
-    const T* vp[NI];
+    const C* kp[NI];
+    const C* vp[NI];
 #pragma unroll
     for (int r = 0; r < NI; ++r) kp[r] = vp[r] = nullptr;
-    gather_to(j, [&](int r, const T* k, const T* v) {
+    gather_to(j, [&](int r, const C* k, const C* v) {
       kp[r] = k;
       vp[r] = v;
     });
@@ -510,12 +581,14 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerEu, kWavesPerEu))) void paged_prefil
   //   V block db:  vb[h] + ((db ^ vt) << 6)   (row + 8h flips only swizzle bits 0-1),
   // which keeps 5 VGPRs live instead of 16; other head dims keep a table.
   uint32_t koff[DC], voff[DB][2];
+  if constexpr (!kQ8) {
 #pragma unroll
-  for (int c = 0; c < DC; ++c) koff[c] = 2 * L::at(col, 16 * c + 8 * half);
+    for (int c = 0; c < DC; ++c) koff[c] = 2 * L::at(col, 16 * c + 8 * half);
 #pragma unroll
-  for (int db = 0; db < DB; ++db)
+    for (int db = 0; db < DB; ++db)
 #pragma unroll
-    for (int h = 0; h < 2; ++h) voff[db][h] = 2 * L::at(tr_row + 8 * h, 32 * db + tr_col);
+      for (int h = 0; h < 2; ++h) voff[db][h] = 2 * L::at(tr_row + 8 * h, 32 * db + tr_col);
+  }
   const uint32_t kb0 = col * 256 + ((half ^ (L::swizzle(col) & 1)) << 4);
   const uint32_t kt = L::swizzle(col) >> 1;
   const uint32_t vb0 = tr_row * 256 + (((tr_col >> 3) ^ (L::swizzle(tr_row) & 3)) << 4) + (tr_col & 7) * 2;
@@ -531,17 +604,46 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerEu, kWavesPerEu))) void paged_prefil
     else return voff[db][h];
   };
 
+  // 8-bit cache: K operand reads start at row `col`, chunk `half`; transposed V reads at
+  // key 4half + {0..3} or 8 + 4half + {0..3}, dims 16 * (lane / 16 % 2) + 8 * (lane % 2).
+  const uint32_t kb8 = col * D + 16 * (half ^ Lds8<D>::swizzle(col));
+  const int tr8_row = ((lane >> 1) & 3) + 4 * half + 8 * ((lane >> 3) & 1);
+  const uint32_t vb8 = tr8_row * D + 16 * (((lane >> 4) & 1) ^ Lds8<D>::swizzle(tr8_row)) + 8 * (lane & 1);
+  // Scales of a sub-block's two 16-key halves: K's with the softmax scale, V's (v_scale).
+  float kl[2], vscale[2], pscale[2];
+  auto scales_of = [&](int j) {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int page = page_of(min(j * kSB + 16 * t, end - 1));
+      const uint32_t e = __builtin_amdgcn_readfirstlane((uint32_t)scale_lds[page - tbl_base]);
+      // (0, a page never written, would make NaN of masked scores)
+      kl[t] = __uint_as_float(__builtin_amdgcn_readfirstlane(
+          __float_as_uint(q8_scale(max((int)(e & 255), kLeastExponent)) * a.scale_log2)));
+      v_scale<T>((int)(e >> 8), vscale[t], pscale[t]);
+    }
+  };
+
   // P^T B-operands of scores `st` (already masked, m current): per 16-key
   // chunk c, elements 8c .. 8c+7 of st, i.e. keys 16c + 4half + {0..3} and
   // 16c + 8 + 4half + {0..3}.
   auto probs = [&](const f32x16& st, u32x4 (&pop)[2]) {
     float p[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) p[i] = fast_exp2(fmaf(st[i], a.scale_log2, -m));
+    for (int i = 0; i < 16; ++i) p[i] = fast_exp2(fmaf(st[i], kQ8 ? kl[i >> 3] : a.scale_log2, -m));
+    float w[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) w[i] = p[i];
+    if constexpr (kQ8 && std::is_same<T, f16_t>::value) {
+      // (wave-uniform, and true only for pages of values past 57344)
+      if (pscale[0] != 1.f || pscale[1] != 1.f) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) w[i] *= pscale[i >> 3];
+      }
+    }
 #pragma unroll
     for (int c = 0; c < 2; ++c)
-      pop[c] = u32x4{pack2<T>(p[8 * c], p[8 * c + 1]), pack2<T>(p[8 * c + 2], p[8 * c + 3]),
-                     pack2<T>(p[8 * c + 4], p[8 * c + 5]), pack2<T>(p[8 * c + 6], p[8 * c + 7])};
+      pop[c] = u32x4{pack2<T>(w[8 * c], w[8 * c + 1]), pack2<T>(w[8 * c + 2], w[8 * c + 3]),
+                     pack2<T>(w[8 * c + 4], w[8 * c + 5]), pack2<T>(w[8 * c + 6], w[8 * c + 7])};
     // Pairwise sum: a dependency chain of 4 adds instead of 16.
 #pragma unroll
     for (int w = 1; w < 16; w *= 2)
@@ -564,7 +666,18 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerEu, kWavesPerEu))) void paged_prefil
   auto row_max = [&](int j, f32x16& st, auto masked_c) {
     const int k0 = j * kSB;
     float mx = -INFINITY;
-    if constexpr (!decltype(masked_c)::value) {
+    if constexpr (kQ8) {
+      if constexpr (decltype(masked_c)::value) {
+        const int bound = (q_ok ? min(qpos, end - 1) : -1) - k0 - 4 * half;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) st[e] = 8 * (e >> 2) + (e & 3) <= bound ? st[e] : -INFINITY;
+      }
+      // Each half by its page's scale: the result is in the log2 domain.
+      float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int e = 0; e < 16; ++e) top[e >> 3] = fmaxf(top[e >> 3], st[e]);
+      mx = fmaxf(top[0] * kl[0], top[1] * kl[1]);
+    } else if constexpr (!decltype(masked_c)::value) {
 #pragma unroll
       for (int e = 0; e < 16; ++e) mx = fmaxf(mx, st[e]);
     } else {
@@ -588,9 +701,9 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerEu, kWavesPerEu))) void paged_prefil
                                                        false, false);
       mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
     }
-    const float mcand = mx * a.scale_log2;
-    if (__any(mcand > m + 8.f)) {
-      const float mnew = fmaxf(m, mcand);
+    const float mcand = kQ8 ? mx : mx * a.scale_log2;
+    if (__any(mcand > m + (kQ8 ? Weights<T>::kSlack : 8.f))) {
+      const float mnew = fmaxf(m, kQ8 ? mcand - Weights<T>::kLift : mcand);
       const float corr = fast_exp2(m - mnew);
       lsum *= corr;
 #pragma unroll
@@ -628,6 +741,80 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerEu, kWavesPerEu))) void paged_prefil
     if (full_share) vm_wait<kDmaPerStep>();
     else vm_wait<2 * (NI - 1)>();
   };
+  // A step over the 8-bit cache: the stages at kd and vd hold sub-block j.
+  // Accumulators that are NaN by a value that their query sees: bit e of [db][thread].
+  __shared__ uint16_t poison_lds[kQ8 ? DB : 1][kQ8 ? kThreads : 1];
+  bool poisoned = false;
+  if constexpr (kQ8) {
+#pragma unroll
+    for (int db = 0; db < DB; ++db) poison_lds[db][tid] = 0;
+  }
+  auto attend8 = [&](int j, const char* kd, const char* vd) __attribute__((always_inline)) {
+    scales_of(j);
+    f32x16 st = f32x16{};
+    auto kread = [&](int c) { return *reinterpret_cast<const u32x4*>(kd + Lds8<D>::chunk(kb8, c)); };
+    u32x4 kop[DC / 2];
+    kop[0] = kread(0);
+#pragma unroll
+    for (int c = 0; c < DC / 2; ++c) {
+      if (c + 1 < DC / 2) kop[c + 1] = kread(c + 1);
+      st = Mfma<T>::run(MfmaQ8<T>::widen(kop[c][0], kop[c][1], 1.f, 1.f), qop[2 * c], st);
+      st = Mfma<T>::run(MfmaQ8<T>::widen(kop[c][2], kop[c][3], 1.f, 1.f), qop[2 * c + 1], st);
+    }
+    mask_max(j, st);
+    u32x4 pop[2];
+    probs(st, pop);
+    auto vread = [&](int i) { return lds_read_tr8(vd + 16 * (i / DB) * D + Lds8<D>::chunk(vb8, i % DB)); };
+    if (unmasked(j)) {
+      u32x2 vop[2 * DB];
+      vop[0] = vread(0);
+#pragma unroll
+      for (int i = 0; i < 2 * DB; ++i) {
+        if (i + 1 < 2 * DB) vop[i + 1] = vread(i + 1);
+        acc[i % DB] = Mfma<T>::run(MfmaQ8<T>::widen(vop[i][0], vop[i][1], vscale[i / DB], vscale[i / DB]),
+                                   pop[i / DB], acc[i % DB]);
+      }
+      return;
+    }
+    // A value that a query does not see must not reach it, and 0 * NaN would: where the
+    // mask is at work, NaN values are taken out of the product, and (rarely) a product of
+    // their places with the mask finds the queries that do see them.
+    uint32_t found = 0;
+#pragma unroll
+    for (int i = 0; i < 2 * DB; ++i) {
+      const u32x2 x = vread(i);
+      const uint32_t b0 = nan_bytes(x[0]), b1 = nan_bytes(x[1]);
+      found |= b0 | b1;
+      acc[i % DB] = Mfma<T>::run(MfmaQ8<T>::widen(x[0] & ~(b0 * 0xFF), x[1] & ~(b1 * 0xFF), vscale[i / DB],
+                                                  vscale[i / DB]),
+                                 pop[i / DB], acc[i % DB]);
+    }
+    if (!__any(found != 0)) return;
+    const int bound = (q_ok ? min(qpos, end - 1) : -1) - j * kSB - 4 * half;
+    u32x4 seen[2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = 16 * c + 8 * (i >> 1) + 2 * (i & 1);
+        seen[c][i] = pack2<bf16_t>(key <= bound ? 1.f : 0.f, key + 1 <= bound ? 1.f : 0.f);
+      }
+#pragma unroll 1
+    for (int db = 0; db < DB; ++db) {
+      f32x16 hit = {};
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const u32x2 x = lds_read_tr8(vd + 16 * c * D + Lds8<D>::chunk(vb8, db));
+        hit = Mfma<bf16_t>::run(
+            MfmaQ8<bf16_t>::widen(nan_bytes(x[0]) * 0x38, nan_bytes(x[1]) * 0x38, 1.f, 1.f), seen[c], hit);
+      }
+      uint32_t bits = 0;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) bits |= (hit[e] > 0.f ? 1u : 0u) << e;
+      poison_lds[db][tid] |= (uint16_t)bits;
+    }
+    poisoned = true;
+  };
   if (j0 < nsub) {
     dma(j0, H0{});
     if (j0 + 1 < nsub) dma(j0 + 1, H1{});
@@ -641,6 +828,10 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerEu, kWavesPerEu))) void paged_prefil
       if (j >= nsub_w) return;
       const char* kd = reinterpret_cast<const char*>(ks[h]);
       f32x16 st = f32x16{};
+      if constexpr (kQ8) {
+        attend8(j, kd, reinterpret_cast<const char*>(vs[h]));
+        return;
+      }
       // Each operand is read one MFMA ahead of its use, so a read's latency
       // overlaps the MFMA before it (two in flight per wave at most, which
       // the register budget of three waves per SIMD allows).
@@ -686,6 +877,16 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerEu, kWavesPerEu))) void paged_prefil
     }
   }
   lsum += shfl_xor_f32(lsum, 32);
+  if constexpr (kQ8) {
+    if (poisoned) {
+#pragma unroll
+      for (int db = 0; db < DB; ++db) {
+        const uint32_t bits = poison_lds[db][tid];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[db][e] = bits >> e & 1 ? NAN : acc[db][e];
+      }
+    }
+  }
   if (tile_sub > run) {
     // This split's (m, l, O) in the accumulator's own layout (1 KiB per wave
     // store); paged_prefill_merge_kernel reads it back the same way.
@@ -849,12 +1050,12 @@ __global__ __launch_bounds__(1024) void prefill_order_kernel(const int32_t* cu, 
   }
 }
 
-template <typename T, int MODE>
+template <typename T, typename C, int MODE>
 bool launch_prefill_d(int d, dim3 grid, hipStream_t s, const PrefillArgs& a) {
   switch (d) {
 #define VRH_D(DV)                                                                          \
   case DV:                                                                                 \
-    hipLaunchKernelGGL((paged_prefill_kernel<T, DV, MODE>), grid, dim3(kThreads), 0, s, a); \
+    hipLaunchKernelGGL((paged_prefill_kernel<T, C, DV, MODE>), grid, dim3(kThreads), 0, s, a); \
     return true;
     VRH_D(32)
     VRH_D(64)
@@ -865,10 +1066,10 @@ bool launch_prefill_d(int d, dim3 grid, hipStream_t s, const PrefillArgs& a) {
   }
 }
 
-template <typename T>
+template <typename T, typename C = T>
 bool launch_prefill(int d, dim3 grid, hipStream_t s, const PrefillArgs& a) {
-  if (a.bs_shift >= 0) return launch_prefill_d<T, kShift>(d, grid, s, a);
-  return launch_prefill_d<T, kDiv>(d, grid, s, a);
+  if (a.bs_shift >= 0) return launch_prefill_d<T, C, kShift>(d, grid, s, a);
+  return launch_prefill_d<T, C, kDiv>(d, grid, s, a);
 }
 
 }  // namespace
@@ -964,6 +1165,130 @@ extern "C" size_t vrh_paged_prefill_split_workspace_bytes(int64_t num_seqs, int6
              split_slot_bytes(head_dim);
 }
 
+namespace {
+// A packed call that runs on MFMA tiles, whatever the cache's type: `a` holds its
+// pointers, strides and scales, `rows_bytes` the room of the decode rows' partials at
+// the workspace's start.
+struct TileCall {
+  const char* who;
+  int dtype;
+  bool q8;
+  PrefillArgs a;
+  int64_t num_seqs, total_q;
+  int32_t max_seqlen_q, q_heads, kv_heads, head_dim, block_size, table_width;
+  bool route_decode;  // the workspace has room for the decode rows and the order
+  size_t rows_bytes;
+  void* workspace;
+  size_t workspace_bytes;
+};
+
+// launch_rows(expand_e, later, later_blocks) launches the decode rows of sequences with
+// at most expand_e queries; with `later` their merge may be left to the tiles'.
+template <typename Rows>
+int run_tiles(const TileCall& c, hipStream_t s, Rows&& launch_rows) {
+  const int dtype = c.dtype;
+  const int64_t num_seqs = c.num_seqs, total_q = c.total_q;
+  const int32_t max_seqlen_q = c.max_seqlen_q, q_heads = c.q_heads, kv_heads = c.kv_heads;
+  const int32_t head_dim = c.head_dim, block_size = c.block_size, table_width = c.table_width;
+  const bool route_decode = c.route_decode;
+  void* const workspace = c.workspace;
+  const int route_q = decode_route_q(max_seqlen_q);
+  VRH_CHECK_ARG(max_seqlen_q >= 1, "%s: max_seqlen_q must be positive", c.who);
+  VRH_CHECK_ARG(q_heads <= 65535, "%s: too many heads", c.who);
+  PrefillArgs a = c.a;
+  a.group = q_heads / kv_heads;
+  a.block_size = block_size;
+  a.bs_shift = (block_size & (block_size - 1)) == 0 ? __builtin_ctz((unsigned)block_size) : -1;
+  a.table_width = table_width;
+  // A lone sequence with more than kExactQ queries needs no decode launch: the
+  // tiles handle it whatever its query count turns out to be.
+  const bool route_rows = route_decode && !(num_seqs == 1 && max_seqlen_q > kExactQ);
+  a.skip_q = route_rows ? route_q : 0;
+  {
+    // Rows one staging instruction covers: 64 lanes of 16 bytes over rows of
+    // `chunks` chunks; the fast addressing needs them on one page.
+    const int chunks = c.q8 ? head_dim / 16 : head_dim / 8;
+    const bool pow2_chunks = (chunks & (chunks - 1)) == 0;
+    a.uniform_pages = pow2_chunks && a.bs_shift >= 0 && block_size % (64 / chunks) == 0;
+  }
+  a.same_kv32 = a.k_block == a.v_block && a.k_token == a.v_token && a.k_block >= 0 &&
+                a.k_block < (1ll << 31) && a.k_token >= 0 && a.k_token < (1ll << 31);
+  a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)head_dim));
+  a.num_seqs = num_seqs;
+  a.kv_heads = kv_heads;
+  // No sequence has more than total_q queries, so a max_seqlen_q that only bounds
+  // them from above (up to INT32_MAX) costs no tiles and is not refused.
+  const int64_t qblocks = ceil_div64(std::min<int64_t>(max_seqlen_q, total_q) * a.group, kBM);
+  VRH_CHECK_ARG(qblocks <= (1 << 24), "%s: too many work items", c.who);
+  a.qblocks = (int32_t)qblocks;
+  // Up to 64 sequences are ranked inside the kernel (also without a
+  // workspace); larger batches use the ordering kernel and the workspace.
+  a.order = nullptr;
+  a.rank_in_kernel = num_seqs > 1 && num_seqs <= 64;
+  // Key splits when the workspace has room for their partials (after the
+  // decode partials and the dispatch order).
+  a.splits = 1;
+  const int64_t cap_tiles = most_tiles(num_seqs, total_q, max_seqlen_q, a.group);
+  a.cap_tiles = (int32_t)std::min<int64_t>(cap_tiles, 1 << 30);
+  a.target = target_items(head_dim);
+  a.part_acc = a.part_ml = nullptr;
+  a.any_split = nullptr;
+  if (route_decode) {
+    const size_t base =
+        (c.rows_bytes + (size_t)num_seqs * sizeof(int32_t) + 255) / 256 * 256;
+    const int32_t splits = most_splits(num_seqs, total_q, max_seqlen_q, q_heads, kv_heads, head_dim,
+                                       block_size, table_width);
+    const size_t slots = (size_t)cap_tiles * kv_heads * splits;
+    if (splits > 1 && c.workspace_bytes >= base + slots * split_slot_bytes(head_dim)) {
+      a.splits = splits;
+      a.rank_in_kernel = 1;  // the runs follow from the same per-lane lengths
+      a.part_acc = reinterpret_cast<float*>(static_cast<char*>(workspace) + base);
+      a.part_ml = a.part_acc + slots * kBM * head_dim;
+      // In the dispatch order's place, which a batch ranked in the kernel does not use.
+      a.any_split = reinterpret_cast<int32_t*>(
+          static_cast<char*>(workspace) + c.rows_bytes);
+    }
+  }
+  a.compact = a.rank_in_kernel && kv_heads % 8 == 0;
+  // With every sequence routed to the decode kernel (max_seqlen_q <= the
+  // routed query count) the MFMA launch, and its ordering, would have no work.
+  const bool mfma_work = a.skip_q < max_seqlen_q;
+  if (mfma_work && route_decode && num_seqs > 1 && num_seqs <= kOrderMax && !a.rank_in_kernel) {
+    int32_t* order = reinterpret_cast<int32_t*>(
+        static_cast<char*>(workspace) + c.rows_bytes);
+    hipLaunchKernelGGL(prefill_order_kernel, dim3(1), dim3(1024), 0, s, a.cu, a.lengths,
+                       (int32_t)num_seqs, a.skip_q, (int64_t)table_width * block_size, order);
+    a.order = order;
+  }
+  const int64_t groups = num_seqs * kv_heads * a.splits;
+  const int64_t launched = a.compact ? cap_tiles * kv_heads * a.splits
+                                     : (groups + 7) / 8 * 8 * (int64_t)a.qblocks;
+  VRH_CHECK_ARG(launched < (1ll << 31), "%s: too many work items", c.who);
+  if (mfma_work) {
+    const dim3 grid((unsigned)launched);
+    const bool ok =
+        dtype == VRH_DTYPE_BF16
+            ? (c.q8 ? launch_prefill<bf16_t, e4m3_t>(head_dim, grid, s, a) : launch_prefill<bf16_t>(head_dim, grid, s, a))
+            : (c.q8 ? launch_prefill<f16_t, e4m3_t>(head_dim, grid, s, a) : launch_prefill<f16_t>(head_dim, grid, s, a));
+    VRH_CHECK_ARG(ok, "%s: no kernel for head_dim %d", c.who, head_dim);
+  }
+  DecodeArgs rows = {};  // merged with the tiles' runs when the call may have any
+  unsigned decode_blocks = 0;
+  if (route_rows) {
+    const int rc = launch_rows(route_q, a.splits > 1 ? &rows : nullptr, &decode_blocks);
+    if (rc != VRH_OK) return rc;
+  }
+  if (a.splits > 1) {
+    const unsigned tile_blocks = (unsigned)(head_dim / 32 * kWaves * cap_tiles * kv_heads);
+    if (dtype == VRH_DTYPE_BF16)
+      launch_prefill_merge<bf16_t>(head_dim, tile_blocks, s, a, rows, decode_blocks);
+    else
+      launch_prefill_merge<f16_t>(head_dim, tile_blocks, s, a, rows, decode_blocks);
+  }
+  VRH_RETURN_LAUNCH(c.who);
+}
+}  // namespace
+
 extern "C" int vrh_paged_prefill(int dtype, void* out, const void* q, const void* key_cache,
                                  const void* value_cache, const int32_t* block_tables,
                                  const int32_t* context_lengths, const int32_t* cu_seqlens_q,
@@ -1012,9 +1337,10 @@ extern "C" int vrh_paged_prefill(int dtype, void* out, const void* q, const void
                            exact ? decode_part_bytes(num_seqs, max_seqlen_q, q_heads, head_dim) : 0,
                            s, "vrh_paged_prefill");
   }
-  VRH_CHECK_ARG(max_seqlen_q >= 1, "vrh_paged_prefill: max_seqlen_q must be positive");
-  VRH_CHECK_ARG(q_heads <= 65535, "vrh_paged_prefill: too many heads");
-  PrefillArgs a = {};  // pointers not set below are null
+  TileCall c = {};
+  c.who = "vrh_paged_prefill";
+  c.dtype = dtype;
+  PrefillArgs& a = c.a;
   a.out = out;
   a.q = q;
   a.k = key_cache;
@@ -1033,115 +1359,62 @@ extern "C" int vrh_paged_prefill(int dtype, void* out, const void* q, const void
   a.v_token = v_token_stride;
   a.v_head = v_head_stride;
   a.table_stride = table_stride;
-  a.group = q_heads / kv_heads;
-  a.block_size = block_size;
-  a.bs_shift = (block_size & (block_size - 1)) == 0 ? __builtin_ctz((unsigned)block_size) : -1;
-  a.table_width = table_width;
-  // A lone sequence with more than kExactQ queries needs no decode launch: the
-  // tiles handle it whatever its query count turns out to be.
-  const bool route_rows = route_decode && !(num_seqs == 1 && max_seqlen_q > kExactQ);
-  a.skip_q = route_rows ? route_q : 0;
-  {
-    // Rows one staging instruction covers: 64 lanes of 16 bytes over rows of
-    // head_dim / 8 chunks; the fast addressing needs them on one page.
-    const int chunks = head_dim / 8;
-    const bool pow2_chunks = (chunks & (chunks - 1)) == 0;
-    a.uniform_pages = pow2_chunks && a.bs_shift >= 0 && block_size % (64 / chunks) == 0;
-  }
-  a.same_kv32 = k_block_stride == v_block_stride &&
-                k_token_stride == v_token_stride && k_block_stride >= 0 &&
-                k_block_stride < (1ll << 31) && k_token_stride >= 0 &&
-                k_token_stride < (1ll << 31);
-  a.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)head_dim));
-  a.num_seqs = num_seqs;
-  a.kv_heads = kv_heads;
-  // No sequence has more than total_q queries, so a max_seqlen_q that only bounds
-  // them from above (up to INT32_MAX) costs no tiles and is not refused.
-  const int64_t qblocks = ceil_div64(std::min<int64_t>(max_seqlen_q, total_q) * a.group, kBM);
-  VRH_CHECK_ARG(qblocks <= (1 << 24), "vrh_paged_prefill: too many work items");
-  a.qblocks = (int32_t)qblocks;
-  // Up to 64 sequences are ranked inside the kernel (also without a
-  // workspace); larger batches use the ordering kernel and the workspace.
-  a.order = nullptr;
-  a.rank_in_kernel = num_seqs > 1 && num_seqs <= 64;
-  // Key splits when the workspace has room for their partials (after the
-  // decode partials and the dispatch order).
-  a.splits = 1;
-  const int64_t cap_tiles = most_tiles(num_seqs, total_q, max_seqlen_q, a.group);
-  a.cap_tiles = (int32_t)std::min<int64_t>(cap_tiles, 1 << 30);
-  a.target = target_items(head_dim);
-  a.part_acc = a.part_ml = nullptr;
-  a.any_split = nullptr;
-  if (route_decode) {
-    const size_t base =
-        (vrh_paged_prefill_workspace_bytes(num_seqs, max_seqlen_q, q_heads, head_dim) + 255) / 256 * 256;
-    const int32_t splits = most_splits(num_seqs, total_q, max_seqlen_q, q_heads, kv_heads, head_dim,
-                                       block_size, table_width);
-    const size_t slots = (size_t)cap_tiles * kv_heads * splits;
-    if (splits > 1 && workspace_bytes >= base + slots * split_slot_bytes(head_dim)) {
-      a.splits = splits;
-      a.rank_in_kernel = 1;  // the runs follow from the same per-lane lengths
-      a.part_acc = reinterpret_cast<float*>(static_cast<char*>(workspace) + base);
-      a.part_ml = a.part_acc + slots * kBM * head_dim;
-      // In the dispatch order's place, which a batch ranked in the kernel does not use.
-      a.any_split = reinterpret_cast<int32_t*>(
-          static_cast<char*>(workspace) + decode_part_bytes(num_seqs, max_seqlen_q, q_heads, head_dim));
-    }
-  }
-  a.compact = a.rank_in_kernel && kv_heads % 8 == 0;
-  // With every sequence routed to the decode kernel (max_seqlen_q <= the
-  // routed query count) the MFMA launch, and its ordering, would have no work.
-  const bool mfma_work = a.skip_q < max_seqlen_q;
-  if (mfma_work && route_decode && num_seqs > 1 && num_seqs <= kOrderMax && !a.rank_in_kernel) {
-    int32_t* order = reinterpret_cast<int32_t*>(
-        static_cast<char*>(workspace) + decode_part_bytes(num_seqs, max_seqlen_q, q_heads, head_dim));
-    hipLaunchKernelGGL(prefill_order_kernel, dim3(1), dim3(1024), 0, s, cu_seqlens_q,
-                       context_lengths, (int32_t)num_seqs, a.skip_q,
-                       (int64_t)table_width * block_size, order);
-    a.order = order;
-  }
-  const int64_t groups = num_seqs * kv_heads * a.splits;
-  const int64_t launched = a.compact ? cap_tiles * kv_heads * a.splits
-                                     : (groups + 7) / 8 * 8 * (int64_t)a.qblocks;
-  VRH_CHECK_ARG(launched < (1ll << 31), "vrh_paged_prefill: too many work items");
-  if (mfma_work) {
-    const bool ok = dtype == VRH_DTYPE_BF16
-                        ? launch_prefill<bf16_t>(head_dim, dim3((unsigned)launched), s, a)
-                        : launch_prefill<f16_t>(head_dim, dim3((unsigned)launched), s, a);
-    VRH_CHECK_ARG(ok, "vrh_paged_prefill: no kernel for head_dim %d", head_dim);
-  }
-  DecodeArgs rows = {};  // merged with the tiles' runs when the call may have any
-  unsigned decode_blocks = 0;
-  if (route_rows) {
-    // Short sequences of the packed batch: one split-KV decode row per query
-    // (row r is query r % route_q of sequence r / route_q).
-    const int rc = vrh_decode_rows(
+  c.num_seqs = num_seqs;
+  c.total_q = total_q;
+  c.max_seqlen_q = max_seqlen_q;
+  c.q_heads = q_heads;
+  c.kv_heads = kv_heads;
+  c.head_dim = head_dim;
+  c.block_size = block_size;
+  c.table_width = table_width;
+  c.route_decode = route_decode;
+  c.rows_bytes = decode_part_bytes(num_seqs, max_seqlen_q, q_heads, head_dim);
+  c.workspace = workspace;
+  c.workspace_bytes = workspace_bytes;
+  // Short sequences of the packed batch: one split-KV decode row per query (row r is
+  // query r % E of sequence r / E).
+  return run_tiles(c, s, [&](int e, DecodeArgs* later, unsigned* later_blocks) {
+    return vrh_decode_rows(
         dtype, out, q, key_cache, value_cache, block_tables, context_lengths, cu_seqlens_q,
-        (int32_t)num_seqs, route_q, num_seqs * route_q, q_heads, kv_heads, head_dim,
-        block_size, table_width, table_stride, q_token_stride, q_head_stride, out_token_stride,
-        out_head_stride, k_block_stride, k_token_stride, k_head_stride, v_block_stride,
-        v_token_stride, v_head_stride, 0, workspace,
-        decode_part_bytes(num_seqs, max_seqlen_q, q_heads, head_dim), s, "vrh_paged_prefill",
-        a.splits > 1 ? &rows : nullptr, &decode_blocks);
-    if (rc != VRH_OK) return rc;
-  }
-  if (a.splits > 1) {
-    const unsigned tile_blocks = (unsigned)(head_dim / 32 * kWaves * cap_tiles * kv_heads);
-    if (dtype == VRH_DTYPE_BF16)
-      launch_prefill_merge<bf16_t>(head_dim, tile_blocks, s, a, rows, decode_blocks);
-    else
-      launch_prefill_merge<f16_t>(head_dim, tile_blocks, s, a, rows, decode_blocks);
-  }
-  VRH_RETURN_LAUNCH("vrh_paged_prefill");
+        (int32_t)num_seqs, e, num_seqs * e, q_heads, kv_heads, head_dim, block_size, table_width,
+        table_stride, q_token_stride, q_head_stride, out_token_stride, out_head_stride,
+        k_block_stride, k_token_stride, k_head_stride, v_block_stride, v_token_stride,
+        v_head_stride, 0, workspace, c.rows_bytes, s, "vrh_paged_prefill", later, later_blocks);
+  });
 }
 
 // ---------------------------------------------------------------- 8-bit cache
-extern "C" size_t vrh_paged_prefill_q8_workspace_bytes(int64_t num_seqs, int64_t total_q,
+namespace {
+size_t rows_bytes_q8(int64_t num_seqs, int32_t max_seqlen_q, int32_t q_heads, int32_t head_dim,
+                     int32_t block_size, int32_t table_width) {
+  return (vrh_paged_decode_q8_workspace_bytes(num_seqs * decode_route_q(max_seqlen_q), q_heads, head_dim,
+                                              block_size, table_width, 0) +
+          255) / 256 * 256;
+}
+bool tiles_q8(int dtype, int32_t head_dim, int32_t block_size) {
+  // Scales are looked up once per 16 keys.
+  return (dtype == VRH_DTYPE_BF16 || dtype == VRH_DTYPE_F16) && tile_head_dim(head_dim) &&
+         block_size >= 16 && block_size % 16 == 0 && block_size <= 65536;
+}
+}  // namespace
+
+extern "C" size_t vrh_paged_prefill_q8_workspace_bytes(int dtype, int64_t num_seqs, int64_t total_q,
                                                        int32_t max_seqlen_q, int32_t q_heads,
                                                        int32_t kv_heads, int32_t head_dim,
                                                        int32_t block_size, int32_t table_width) {
-  return vrh_paged_decode_q8_workspace_bytes(num_seqs * decode_route_q(max_seqlen_q), q_heads, head_dim,
-                                             block_size, table_width, 0);
+  if (num_seqs <= 0 || total_q <= 0 || max_seqlen_q <= 0 || q_heads <= 0 || kv_heads <= 0 || head_dim <= 0 ||
+      block_size <= 0 || table_width < 0)
+    return 0;
+  const bool tiles = tiles_q8(dtype, head_dim, block_size);
+  if (!tiles && max_seqlen_q > kExactQ) return 0;
+  const size_t rows = rows_bytes_q8(num_seqs, max_seqlen_q, q_heads, head_dim, block_size, table_width);
+  if (!tiles) return rows;
+  const size_t base = (rows + (size_t)num_seqs * sizeof(int32_t) + 255) / 256 * 256;
+  const int32_t splits = most_splits(num_seqs, total_q, max_seqlen_q, q_heads, kv_heads, head_dim,
+                                     block_size, table_width);
+  if (splits <= 1) return base;
+  return base + (size_t)most_tiles(num_seqs, total_q, max_seqlen_q, q_heads / kv_heads) * kv_heads * splits *
+                    split_slot_bytes(head_dim);
 }
 
 extern "C" int vrh_paged_prefill_q8(int dtype, void* out, const void* q, const void* key_cache,
@@ -1167,8 +1440,70 @@ extern "C" int vrh_paged_prefill_q8(int dtype, void* out, const void* q, const v
                     q_token_stride, q_head_stride, out_token_stride, out_head_stride,
                     cache_block_stride, cache_token_stride, cache_head_stride, scale_block_stride,
                     scale_head_stride};
-  const bool exact = max_seqlen_q <= kExactQ;
-  return vrh_decode_rows_q8(c, cu_seqlens_q, (int32_t)num_seqs, exact ? max_seqlen_q : 0,
-                            exact ? num_seqs * max_seqlen_q : total_q, 0, workspace, workspace_bytes,
-                            !exact, (hipStream_t)stream, who);
+  hipStream_t s = (hipStream_t)stream;
+  VRH_CHECK_ARG(q_heads >= 1 && kv_heads >= 1 && q_heads % kv_heads == 0,
+                "%s: query heads must be a positive multiple of KV heads", who);
+  VRH_CHECK_ARG(block_size >= 1 && table_width >= 0 && num_blocks >= 1 && head_dim >= 1,
+                "%s: bad block_size/table_width/num_blocks/head_dim", who);
+  bool mfma = tiles_q8(dtype, head_dim, block_size);
+  for (int64_t x : {q_token_stride, q_head_stride}) mfma = mfma && x % 8 == 0;
+  for (int64_t x : {out_token_stride, out_head_stride}) mfma = mfma && x % 4 == 0;
+  for (int64_t x : {cache_block_stride, cache_token_stride, cache_head_stride}) mfma = mfma && x % 16 == 0;
+  for (const void* p : {(const void*)out, q, key_cache, value_cache}) mfma = mfma && (uintptr_t)p % 16 == 0;
+  const size_t need = vrh_paged_prefill_q8_workspace_bytes(dtype, num_seqs, total_q, max_seqlen_q, q_heads,
+                                                           kv_heads, head_dim, block_size, table_width);
+  VRH_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need),
+                "%s: workspace of %zu bytes needed, %zu given", who, need, workspace ? workspace_bytes : (size_t)0);
+  VRH_CHECK_ARG(((uintptr_t)workspace & 255) == 0, "%s: workspace misaligned", who);
+  const size_t rows_bytes = rows_bytes_q8(num_seqs, max_seqlen_q, q_heads, head_dim, block_size, table_width);
+  if (!mfma) {
+    // Every query is a decode row: through the splits of single-query decode (bit for
+    // bit the same) when all sequences are short, otherwise one split per row.
+    const bool exact = max_seqlen_q <= kExactQ;
+    return vrh_decode_rows_q8(c, cu_seqlens_q, (int32_t)num_seqs, exact ? max_seqlen_q : 0,
+                              exact ? num_seqs * max_seqlen_q : total_q, 0, workspace, rows_bytes, !exact, s,
+                              who);
+  }
+  VRH_CHECK_ARG(out && q && key_cache && value_cache && scales && block_tables && context_lengths,
+                "%s: null pointer", who);
+  TileCall t = {};
+  t.who = who;
+  t.dtype = dtype;
+  t.q8 = true;
+  PrefillArgs& a = t.a;
+  a.out = out;
+  a.q = q;
+  a.k = key_cache;
+  a.v = value_cache;
+  a.tables = block_tables;
+  a.lengths = context_lengths;
+  a.cu = cu_seqlens_q;
+  a.q_token = q_token_stride;
+  a.q_head = q_head_stride;
+  a.o_token = out_token_stride;
+  a.o_head = out_head_stride;
+  a.k_block = a.v_block = cache_block_stride;
+  a.k_token = a.v_token = cache_token_stride;
+  a.k_head = a.v_head = cache_head_stride;
+  a.table_stride = table_stride;
+  a.scales = (const uint8_t*)scales;
+  a.s_block = scale_block_stride;
+  a.s_head = scale_head_stride;
+  a.num_blocks = num_blocks;
+  t.num_seqs = num_seqs;
+  t.total_q = total_q;
+  t.max_seqlen_q = max_seqlen_q;
+  t.q_heads = q_heads;
+  t.kv_heads = kv_heads;
+  t.head_dim = head_dim;
+  t.block_size = block_size;
+  t.table_width = table_width;
+  t.route_decode = true;
+  t.rows_bytes = rows_bytes;
+  t.workspace = workspace;
+  t.workspace_bytes = workspace_bytes;
+  return run_tiles(t, s, [&](int e, DecodeArgs*, unsigned*) {
+    return vrh_decode_rows_q8(c, cu_seqlens_q, (int32_t)num_seqs, e, num_seqs * e, 0, workspace, rows_bytes,
+                              false, s, who);
+  });
 }

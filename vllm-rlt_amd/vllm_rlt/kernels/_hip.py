@@ -101,7 +101,7 @@ SIGNATURES: dict[str, tuple[object, list]] = {
          _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I32, _P, _SZ, _P],
     ),
     "vrh_paged_prefill_q8_workspace_bytes": (
-        _SZ, [_I64, _I64, _I32, _I32, _I32, _I32, _I32, _I32]
+        _SZ, [_INT, _I64, _I64, _I32, _I32, _I32, _I32, _I32, _I32]
     ),
     "vrh_paged_prefill_q8": (
         _INT,

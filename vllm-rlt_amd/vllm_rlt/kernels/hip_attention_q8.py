@@ -217,8 +217,8 @@ def paged_prefill_attention_q8(q, key_cache, value_cache, scales, block_tables, 
         raise ValueError("max_seqlen_q must be positive")
     lib = library()
     nbytes = lib.vrh_paged_prefill_q8_workspace_bytes(
-        sequences, q.shape[0], max_seqlen_q, q.shape[1], key_cache.shape[2], q.shape[2],
-        key_cache.shape[1], block_tables.shape[1])
+        dtype_code(q.dtype), sequences, q.shape[0], max_seqlen_q, q.shape[1], key_cache.shape[2],
+        q.shape[2], key_cache.shape[1], block_tables.shape[1])
     workspace = _workspace(nbytes, q.device)
     _launch(
         "vrh_paged_prefill_q8", key_cache.device,
