@@ -10,6 +10,11 @@
 //                 kv_finalize, kv_copy_blocks
 //                               the paged KV hot path, with the argument
 //                               meaning of vllm_rlt/kernels/hip_attention.py
+//   vllm_rlt_hip::paged_attention_q8, paged_prefill_q8, kv_append_q8, kv_read_q8
+//                               the same over the 8-bit cache, as
+//                               vllm_rlt/kernels/hip_attention_q8.py
+//   vllm_rlt_hip::sequence_metadata
+//                               a packed step's metadata from lengths on the GPU
 // Each op checks its tensors with TORCH_CHECK (RuntimeError), allocates
 // outputs and workspaces through PyTorch's caching allocator, launches on the
 // current stream of the tensors' device and forwards raw pointers and strides
@@ -22,6 +27,7 @@
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/library.h>
@@ -325,6 +331,215 @@ at::Tensor silu_and_mul(const at::Tensor& gate, const at::Tensor& up) {
   return out;
 }
 
+// ------------------------------------------------------------- 8-bit cache
+// One layer view of the cache: e4m3 [blocks, block_size, Hkv, D], equal strides,
+// scales uint8 [blocks, Hkv, 2].
+void check_cache_q8(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& scales,
+                    const at::Device& device) {
+  for (const auto* c : {&kc, &vc}) {
+    const char* name = c == &kc ? "key_cache" : "value_cache";
+    check_gpu(name, *c, device);
+    TORCH_CHECK(c->dim() == 4 && c->scalar_type() == at::kFloat8_e4m3fn, name,
+                " must be a float8_e4m3fn tensor [blocks, block_size, kv_heads, head_dim]");
+  }
+  TORCH_CHECK(vc.sizes() == kc.sizes() && vc.strides() == kc.strides(),
+              "key_cache and value_cache must have the same shape and strides");
+  TORCH_CHECK(kc.numel() > 0, "the cache is empty");
+  TORCH_CHECK(kc.size(3) == 1 || kc.stride(3) == 1, "caches must have a contiguous head dimension");
+  check_gpu("scales", scales, device);
+  TORCH_CHECK(scales.scalar_type() == at::kByte && scales.dim() == 3 && scales.size(0) == kc.size(0) &&
+                  scales.size(1) == kc.size(2) && scales.size(2) == 2,
+              "scales must be a uint8 tensor [blocks, kv_heads, 2]");
+  TORCH_CHECK(scales.stride(2) == 1, "scales must have a contiguous last dimension");
+}
+
+void check_tables(const at::Tensor& tables, const at::Tensor& lengths, const at::Device& device) {
+  check_int("block_tables", tables, at::kInt, 2, device);
+  check_int("context_lengths", lengths, at::kInt, 1, device);
+  TORCH_CHECK(tables.size(1) <= 1 || tables.stride(1) == 1, "block_tables rows must be contiguous");
+  TORCH_CHECK(lengths.size(0) == tables.size(0),
+              "block_tables and context_lengths must have the same rows");
+}
+
+void check_queries_q8(const at::Tensor& q, const at::Tensor& kc, const at::Tensor& vc,
+                      const at::Tensor& scales, const at::Tensor& tables, const at::Tensor& lengths) {
+  TORCH_CHECK(q.dim() == 3, "q must be [rows, q_heads, head_dim]");
+  dtype_code(q);
+  check_gpu("q", q, q.device());
+  check_cache_q8(kc, vc, scales, q.device());
+  TORCH_CHECK(kc.size(3) == q.size(2), "the cache's head_dim differs from the query head_dim");
+  TORCH_CHECK(q.size(2) <= 256, "the 8-bit cache supports head_dim <= 256");
+  TORCH_CHECK(q.size(1) > 0 && q.size(1) % kc.size(2) == 0,
+              "query heads must be a positive multiple of KV heads");
+  check_tables(tables, lengths, q.device());
+}
+
+at::Tensor scratch(size_t nbytes, const at::Tensor& like) {
+  return nbytes ? at::empty({(int64_t)nbytes}, like.options().dtype(at::kByte)) : at::Tensor();
+}
+void* pointer(const at::Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+at::Tensor paged_attention_q8(const at::Tensor& q_in, const at::Tensor& kc, const at::Tensor& vc,
+                              const at::Tensor& scales, const at::Tensor& tables,
+                              const at::Tensor& lengths_in, int64_t window) {
+  TORCH_CHECK(window >= 0 && window < (1ll << 31), "window must be a nonnegative integer");
+  check_queries_q8(q_in, kc, vc, scales, tables, lengths_in);
+  TORCH_CHECK(tables.size(0) == q_in.size(0),
+              "block_tables and context_lengths must have one row per query row");
+  const c10::DeviceGuard guard(q_in.device());
+  const at::Tensor q = q_in.stride(2) == 1 ? q_in : q_in.contiguous();
+  const at::Tensor lengths = lengths_in.contiguous();
+  at::Tensor out = at::empty(q.sizes(), q.options());
+  const int64_t rows = q.size(0);
+  if (rows == 0) return out;
+  const int32_t heads = (int32_t)q.size(1), dim = (int32_t)q.size(2);
+  const int32_t page = (int32_t)kc.size(1), width = (int32_t)tables.size(1);
+  const size_t nbytes =
+      vrh_paged_decode_q8_workspace_bytes(rows, heads, dim, page, width, (int32_t)window);
+  const at::Tensor workspace = scratch(nbytes, q);
+  check_rc(vrh_paged_decode_q8(dtype_code(q), out.data_ptr(), q.data_ptr(), kc.data_ptr(),
+                               vc.data_ptr(), scales.data_ptr(), tables.data_ptr<int32_t>(),
+                               lengths.data_ptr<int32_t>(), rows, heads, (int32_t)kc.size(2), dim,
+                               kc.size(0), page, width, tables.stride(0), q.stride(0), q.stride(1),
+                               out.stride(0), out.stride(1), kc.stride(0), kc.stride(1),
+                               kc.stride(2), scales.stride(0), scales.stride(1), (int32_t)window,
+                               pointer(workspace), nbytes, stream_of(q)),
+           "vrh_paged_decode_q8");
+  return out;
+}
+
+at::Tensor paged_prefill_q8(const at::Tensor& q_in, const at::Tensor& kc, const at::Tensor& vc,
+                            const at::Tensor& scales, const at::Tensor& tables,
+                            const at::Tensor& lengths_in, const at::Tensor& cu_in,
+                            int64_t max_seqlen_q) {
+  check_queries_q8(q_in, kc, vc, scales, tables, lengths_in);
+  check_int("cu_seqlens_q", cu_in, at::kInt, 1, q_in.device());
+  const int64_t sequences = tables.size(0);
+  TORCH_CHECK(cu_in.size(0) == sequences + 1,
+              "cu_seqlens_q must have one entry more than there are sequences");
+  const c10::DeviceGuard guard(q_in.device());
+  const at::Tensor q = q_in.stride(2) == 1 ? q_in : q_in.contiguous();
+  const at::Tensor lengths = lengths_in.contiguous(), cu = cu_in.contiguous();
+  at::Tensor out = at::empty(q.sizes(), q.options());
+  if (q.size(0) == 0 || sequences == 0) return out;
+  TORCH_CHECK(max_seqlen_q >= 1 && max_seqlen_q < (1ll << 31), "max_seqlen_q must be positive");
+  const int32_t heads = (int32_t)q.size(1), dim = (int32_t)q.size(2), kv = (int32_t)kc.size(2);
+  const int32_t page = (int32_t)kc.size(1), width = (int32_t)tables.size(1);
+  const int code = dtype_code(q);
+  const size_t nbytes = vrh_paged_prefill_q8_workspace_bytes(
+      code, sequences, q.size(0), (int32_t)max_seqlen_q, heads, kv, dim, page, width);
+  const at::Tensor workspace = scratch(nbytes, q);
+  check_rc(vrh_paged_prefill_q8(code, out.data_ptr(), q.data_ptr(), kc.data_ptr(), vc.data_ptr(),
+                                scales.data_ptr(), tables.data_ptr<int32_t>(),
+                                lengths.data_ptr<int32_t>(), cu.data_ptr<int32_t>(), sequences,
+                                q.size(0), (int32_t)max_seqlen_q, heads, kv, dim, kc.size(0), page,
+                                width, tables.stride(0), q.stride(0), q.stride(1), out.stride(0),
+                                out.stride(1), kc.stride(0), kc.stride(1), kc.stride(2),
+                                scales.stride(0), scales.stride(1), pointer(workspace), nbytes,
+                                stream_of(q)),
+           "vrh_paged_prefill_q8");
+  return out;
+}
+
+void kv_append_q8(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& scales,
+                  const at::Tensor& k, const at::Tensor& v, const at::Tensor& tables,
+                  const at::Tensor& lengths_in, const std::optional<at::Tensor>& cu_in) {
+  check_cache_q8(kc, vc, scales, kc.device());
+  for (const auto* t : {&k, &v}) {
+    const char* name = t == &k ? "k" : "v";
+    check_gpu(name, *t, kc.device());
+    TORCH_CHECK(t->dim() == 3 && t->size(1) == kc.size(2) && t->size(2) == kc.size(3), name,
+                " must be [rows, ", kc.size(2), ", ", kc.size(3), "]");
+    TORCH_CHECK(t->size(2) == 1 || t->stride(2) == 1, name, " must have a contiguous head dimension");
+  }
+  const int code = dtype_code(k);
+  TORCH_CHECK(v.scalar_type() == k.scalar_type() && v.sizes() == k.sizes(),
+              "k and v must have the same shape and dtype");
+  check_tables(tables, lengths_in, kc.device());
+  const int64_t sequences = tables.size(0), rows = k.size(0);
+  const c10::DeviceGuard guard(kc.device());
+  at::Tensor cu;
+  if (cu_in.has_value()) {
+    check_int("cu_seqlens_q", *cu_in, at::kInt, 1, kc.device());
+    TORCH_CHECK(cu_in->size(0) == sequences + 1,
+                "cu_seqlens_q must have one entry more than there are sequences");
+    cu = cu_in->contiguous();
+  } else {
+    TORCH_CHECK(rows == sequences, "without cu_seqlens_q, k and v must have one row per sequence");
+  }
+  if (rows == 0 || sequences == 0) return;
+  const at::Tensor lengths = lengths_in.contiguous();
+  check_rc(vrh_kv_append_q8(code, kc.data_ptr(), vc.data_ptr(), scales.data_ptr(), kc.stride(0),
+                            kc.stride(1), kc.stride(2), scales.stride(0), scales.stride(1),
+                            k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), v.stride(0),
+                            v.stride(1), tables.data_ptr<int32_t>(), lengths.data_ptr<int32_t>(),
+                            static_cast<const int32_t*>(pointer(cu)), sequences, rows,
+                            (int32_t)kc.size(2), (int32_t)kc.size(3), kc.size(0),
+                            (int32_t)kc.size(1), (int32_t)tables.size(1), tables.stride(0),
+                            stream_of(kc)),
+           "vrh_kv_append_q8");
+}
+
+std::tuple<at::Tensor, at::Tensor> kv_read_q8(const at::Tensor& kc, const at::Tensor& vc,
+                                              const at::Tensor& scales, const at::Tensor& pages_in,
+                                              at::ScalarType dtype) {
+  check_cache_q8(kc, vc, scales, kc.device());
+  check_int("pages", pages_in, at::kLong, 1, kc.device());
+  const c10::DeviceGuard guard(kc.device());
+  const at::Tensor pages = pages_in.contiguous();
+  const auto options = kc.options().dtype(dtype);
+  at::Tensor keys = at::empty({pages.size(0), kc.size(1), kc.size(2), kc.size(3)}, options);
+  const int code = dtype_code(keys);
+  at::Tensor values = at::empty(keys.sizes(), options);
+  if (pages.size(0) == 0) return {keys, values};
+  check_rc(vrh_kv_read_q8(code, keys.data_ptr(), values.data_ptr(), kc.data_ptr(), vc.data_ptr(),
+                          scales.data_ptr(), kc.stride(0), kc.stride(1), kc.stride(2),
+                          scales.stride(0), scales.stride(1), pages.data_ptr<int64_t>(),
+                          pages.size(0), (int32_t)kc.size(2), (int32_t)kc.size(3), kc.size(0),
+                          (int32_t)kc.size(1), stream_of(kc)),
+           "vrh_kv_read_q8");
+  return {keys, values};
+}
+
+// positions, write blocks, write offsets, write mask, block tables, context lengths,
+// cumulative query lengths.
+using Metadata = std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor,
+                            at::Tensor>;
+Metadata sequence_metadata(const at::Tensor& tables, const at::Tensor& rows_in,
+                           const at::Tensor& lengths_in, const at::Tensor& counts_in, int64_t page,
+                           int64_t tokens, int64_t out_width) {
+  check_int("tables", tables, at::kInt, 2, tables.device());
+  check_int("table_rows", rows_in, at::kLong, 1, tables.device());
+  check_int("context_lengths", lengths_in, at::kInt, 1, tables.device());
+  check_int("query_lengths", counts_in, at::kInt, 1, tables.device());
+  const int64_t n = rows_in.size(0);
+  TORCH_CHECK(lengths_in.size(0) == n && counts_in.size(0) == n,
+              "table_rows, context_lengths and query_lengths must have equal lengths");
+  TORCH_CHECK(tables.size(1) <= 1 || tables.stride(1) == 1, "tables rows must be contiguous");
+  TORCH_CHECK(page >= 1 && tokens >= 0 && out_width >= 0 && page < (1ll << 31) &&
+                  out_width < (1ll << 31),
+              "page must be positive, tokens and out_width nonnegative");
+  const c10::DeviceGuard guard(tables.device());
+  const at::Tensor rows = rows_in.contiguous(), lengths = lengths_in.contiguous(),
+                   counts = counts_in.contiguous();
+  const auto ints = tables.options();
+  const at::Tensor wide = at::empty({3, tokens}, ints.dtype(at::kLong));
+  at::Tensor mask = at::empty({tokens}, ints.dtype(at::kBool));
+  at::Tensor out_tables = at::empty({n, out_width}, ints);
+  const at::Tensor narrow = at::empty({2 * n + 1}, ints);
+  int64_t* w = wide.data_ptr<int64_t>();
+  int32_t* m = narrow.data_ptr<int32_t>();
+  check_rc(vrh_sequence_metadata(tables.data_ptr<int32_t>(), tables.size(0), tables.stride(0),
+                                 rows.data_ptr<int64_t>(), lengths.data_ptr<int32_t>(),
+                                 counts.data_ptr<int32_t>(), w, w + tokens, w + 2 * tokens,
+                                 reinterpret_cast<uint8_t*>(mask.data_ptr<bool>()),
+                                 out_tables.data_ptr<int32_t>(), out_width, m, m + n, n, tokens,
+                                 (int32_t)tables.size(1), (int32_t)out_width, (int32_t)page,
+                                 stream_of(tables)),
+           "vrh_sequence_metadata");
+  return {wide[0], wide[1], wide[2], mask, out_tables, narrow.narrow(0, 0, n), narrow.narrow(0, n, n + 1)};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(vllm_rlt, ops) {
@@ -349,6 +564,18 @@ TORCH_LIBRARY(vllm_rlt_hip, ops) {
           "Tensor tables, int planes) -> ()");
   ops.def("kv_copy_blocks(Tensor(a!) key_cache, Tensor(b!) value_cache, Tensor src_blocks, "
           "Tensor dst_blocks) -> ()");
+  ops.def("paged_attention_q8(Tensor q, Tensor key_cache, Tensor value_cache, Tensor scales, "
+          "Tensor block_tables, Tensor context_lengths, int window=0) -> Tensor");
+  ops.def("paged_prefill_q8(Tensor q, Tensor key_cache, Tensor value_cache, Tensor scales, "
+          "Tensor block_tables, Tensor context_lengths, Tensor cu_seqlens_q, int max_seqlen_q) "
+          "-> Tensor");
+  ops.def("kv_append_q8(Tensor(a!) key_cache, Tensor(b!) value_cache, Tensor(c!) scales, Tensor k, "
+          "Tensor v, Tensor block_tables, Tensor context_lengths, Tensor? cu_seqlens_q=None) -> ()");
+  ops.def("kv_read_q8(Tensor key_cache, Tensor value_cache, Tensor scales, Tensor pages, "
+          "ScalarType dtype) -> (Tensor, Tensor)");
+  ops.def("sequence_metadata(Tensor tables, Tensor table_rows, Tensor context_lengths, "
+          "Tensor query_lengths, int page, int tokens, int out_width) "
+          "-> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(vllm_rlt_hip, CUDA, ops) {
@@ -358,10 +585,15 @@ TORCH_LIBRARY_IMPL(vllm_rlt_hip, CUDA, ops) {
   ops.impl("kv_gather", &kv_gather);
   ops.impl("kv_finalize", &kv_finalize);
   ops.impl("kv_copy_blocks", &kv_copy_blocks);
+  ops.impl("paged_attention_q8", &paged_attention_q8);
+  ops.impl("paged_prefill_q8", &paged_prefill_q8);
+  ops.impl("kv_append_q8", &kv_append_q8);
+  ops.impl("kv_read_q8", &kv_read_q8);
+  ops.impl("sequence_metadata", &sequence_metadata);
 }
 
 // ------------------------------------------------ calls from the Python adapter
-// decode, prefill, append and silu of this module take exactly the plain calls
+// The functions below take exactly the plain calls
 // (ordinary ROCm tensors that pass every check of vllm_rlt/kernels) and answer
 // None to all others, which the adapter then handles, or refuses with its own
 // errors. They skip the adapter's per-call host work: 20.6 us a decode call
@@ -496,11 +728,138 @@ PyObject* py_silu(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// The 8-bit cache's calls and the sequence metadata. Caches and scales as
+// check_cache_q8 wants them; tables and lengths likewise, nothing to copy.
+bool plain_cache_q8(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& scales) {
+  return kc.dim() == 4 && kc.scalar_type() == at::kFloat8_e4m3fn &&
+         vc.scalar_type() == at::kFloat8_e4m3fn && vc.sizes() == kc.sizes() &&
+         vc.strides() == kc.strides() && kc.numel() > 0 && kc.stride(3) == 1 &&
+         scales.scalar_type() == at::kByte && scales.dim() == 3 && scales.size(0) == kc.size(0) &&
+         scales.size(1) == kc.size(2) && scales.size(2) == 2 && scales.stride(2) == 1;
+}
+
+bool plain_ints(const at::Tensor& t, at::ScalarType type, int64_t n) {
+  return t.dim() == 1 && t.scalar_type() == type && t.size(0) == n && t.is_contiguous();
+}
+
+bool plain_tables(const at::Tensor& tables, const at::Tensor& lengths) {
+  return tables.dim() == 2 && tables.scalar_type() == at::kInt &&
+         (tables.size(1) <= 1 || tables.stride(1) == 1) &&
+         plain_ints(lengths, at::kInt, tables.size(0));
+}
+
+// q, key cache, value cache, scales, tables, lengths.
+bool plain_attention_q8(const at::Tensor* const* t) {
+  const at::Tensor &q = *t[0], &kc = *t[1];
+  return q.dim() == 3 && known_dtype(q) && q.stride(2) == 1 && q.size(0) > 0 &&
+         plain_cache_q8(kc, *t[2], *t[3]) && kc.size(3) == q.size(2) && q.size(2) <= 256 &&
+         q.size(1) > 0 && q.size(1) % kc.size(2) == 0 && plain_tables(*t[4], *t[5]);
+}
+
+PyObject* py_decode_q8(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const at::Tensor* t[6];
+  int64_t window;
+  if (n != 7 || !plain_args(args, 6, t) || !plain_attention_q8(t) || !small_int(args[6], &window) ||
+      t[4]->size(0) != t[0]->size(0))
+    return none();
+  return THPVariable_Wrap(unlocked<6>(t, [=](const auto& x) {
+    return paged_attention_q8(x[0], x[1], x[2], x[3], x[4], x[5], window);
+  }));
+  END_HANDLE_TH_ERRORS
+}
+
+PyObject* py_prefill_q8(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const at::Tensor* t[7];
+  int64_t max_q;
+  if (n != 8 || !plain_args(args, 7, t) || !plain_attention_q8(t) || !small_int(args[7], &max_q) ||
+      max_q < 1 || t[4]->size(0) < 1 || !plain_ints(*t[6], at::kInt, t[4]->size(0) + 1))
+    return none();
+  return THPVariable_Wrap(unlocked<7>(t, [=](const auto& x) {
+    return paged_prefill_q8(x[0], x[1], x[2], x[3], x[4], x[5], x[6], max_q);
+  }));
+  END_HANDLE_TH_ERRORS
+}
+
+// key cache, value cache, scales, k, v, tables, lengths, and cumulative lengths or
+// None. True when done.
+PyObject* py_append_q8(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const at::Tensor* t[8];
+  if (n != 8) return none();
+  const bool packed = args[7] != Py_None;
+  if (!plain_args(args, packed ? 8 : 7, t)) return none();
+  const at::Tensor &kc = *t[0], &k = *t[3], &v = *t[4], &tables = *t[5];
+  if (!plain_cache_q8(kc, *t[1], *t[2]) || !known_dtype(k) || v.scalar_type() != k.scalar_type() ||
+      k.dim() != 3 || v.sizes() != k.sizes() || k.size(1) != kc.size(2) || k.size(2) != kc.size(3) ||
+      k.stride(2) != 1 || v.stride(2) != 1 || k.size(0) == 0 || !plain_tables(tables, *t[6]) ||
+      tables.size(0) == 0)
+    return none();
+  if (packed ? !plain_ints(*t[7], at::kInt, tables.size(0) + 1) : tables.size(0) != k.size(0))
+    return none();
+  if (packed)
+    unlocked<8>(t, [](const auto& x) {
+      kv_append_q8(x[0], x[1], x[2], x[3], x[4], x[5], x[6], x[7]);
+    });
+  else
+    unlocked<7>(t, [](const auto& x) {
+      kv_append_q8(x[0], x[1], x[2], x[3], x[4], x[5], x[6], std::nullopt);
+    });
+  Py_RETURN_TRUE;
+  END_HANDLE_TH_ERRORS
+}
+
+template <size_t... I, typename Tuple>
+PyObject* wrap_tuple(Tuple&& x, std::index_sequence<I...>) {
+  PyObject* out = PyTuple_New(sizeof...(I));
+  if (out == nullptr) throw python_error();
+  (PyTuple_SET_ITEM(out, I, THPVariable_Wrap(std::get<I>(std::move(x)))), ...);
+  return out;
+}
+
+// key cache, value cache, scales, pages, dtype.
+PyObject* py_read_q8(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const at::Tensor* t[4];
+  if (n != 5 || !plain_args(args, 4, t) || !THPDtype_Check(args[4]) ||
+      !plain_cache_q8(*t[0], *t[1], *t[2]) || !plain_ints(*t[3], at::kLong, t[3]->numel()))
+    return none();
+  const at::ScalarType dtype = reinterpret_cast<THPDtype*>(args[4])->scalar_type;
+  if (dtype != at::kFloat && dtype != at::kHalf && dtype != at::kBFloat16) return none();
+  return wrap_tuple(unlocked<4>(t, [=](const auto& x) { return kv_read_q8(x[0], x[1], x[2], x[3], dtype); }),
+                    std::make_index_sequence<2>());
+  END_HANDLE_TH_ERRORS
+}
+
+// tables, table rows, context lengths, query lengths, page, tokens, out width.
+PyObject* py_sequence_metadata(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const at::Tensor* t[4];
+  int64_t page, tokens, out_width;
+  if (n != 7 || !plain_args(args, 4, t) || !small_int(args[4], &page) || page < 1 ||
+      !small_int(args[5], &tokens) || !small_int(args[6], &out_width) || t[0]->dim() != 2 ||
+      t[0]->scalar_type() != at::kInt || (t[0]->size(1) > 1 && t[0]->stride(1) != 1) ||
+      !plain_ints(*t[1], at::kLong, t[1]->numel()) || !plain_ints(*t[2], at::kInt, t[1]->numel()) ||
+      !plain_ints(*t[3], at::kInt, t[1]->numel()))
+    return none();
+  return wrap_tuple(unlocked<4>(t, [=](const auto& x) {
+                      return sequence_metadata(x[0], x[1], x[2], x[3], page, tokens, out_width);
+                    }),
+                    std::make_index_sequence<7>());
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef vrh_methods[] = {
     {"decode", (PyCFunction)(void (*)(void))py_decode, METH_FASTCALL, nullptr},
     {"prefill", (PyCFunction)(void (*)(void))py_prefill, METH_FASTCALL, nullptr},
     {"append", (PyCFunction)(void (*)(void))py_append, METH_FASTCALL, nullptr},
     {"silu", (PyCFunction)(void (*)(void))py_silu, METH_FASTCALL, nullptr},
+    {"decode_q8", (PyCFunction)(void (*)(void))py_decode_q8, METH_FASTCALL, nullptr},
+    {"prefill_q8", (PyCFunction)(void (*)(void))py_prefill_q8, METH_FASTCALL, nullptr},
+    {"append_q8", (PyCFunction)(void (*)(void))py_append_q8, METH_FASTCALL, nullptr},
+    {"read_q8", (PyCFunction)(void (*)(void))py_read_q8, METH_FASTCALL, nullptr},
+    {"sequence_metadata", (PyCFunction)(void (*)(void))py_sequence_metadata, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 }  // namespace

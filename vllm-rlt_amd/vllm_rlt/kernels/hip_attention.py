@@ -590,6 +590,12 @@ def sequence_metadata(tables, table_rows, context_lengths, query_lengths, page, 
     cu_seqlens_q)``: the first four per token (``tokens`` of them; those behind the last request
     are masked and 0), then per request the table padded with -1 to ``out_width``, the length,
     and the cumulative query counts. Lengths that do not fit the tables or ``tokens`` are cut."""
+    plain = plain_calls()
+    if plain is not None:
+        metadata = plain.sequence_metadata(tables, table_rows, context_lengths, query_lengths, page,
+                                           tokens, out_width)
+        if metadata is not None:
+            return metadata
     _on_gpu("tables", tables, tables.device)
     device = tables.device
     _check_int("tables", tables, torch.int32, 2, device)
@@ -608,15 +614,18 @@ def sequence_metadata(tables, table_rows, context_lengths, query_lengths, page, 
     block_tables = torch.empty((n, out_width), dtype=torch.int32, device=device)
     narrow = torch.empty(2 * n + 1, dtype=torch.int32, device=device)
     lengths, cu = narrow[:n], narrow[n:]
+    table_rows, context_lengths = table_rows.contiguous(), context_lengths.contiguous()
+    query_lengths = query_lengths.contiguous()
     lib = library()
-    lib.check(
-        lib.vrh_sequence_metadata(
-            tables.data_ptr(), tables.shape[0], tables.stride(0), table_rows.contiguous().data_ptr(),
-            context_lengths.contiguous().data_ptr(), query_lengths.contiguous().data_ptr(),
-            wide[0].data_ptr(), wide[1].data_ptr(), wide[2].data_ptr(), mask.data_ptr(),
-            block_tables.data_ptr(), out_width, lengths.data_ptr(), cu.data_ptr(), n, tokens,
-            tables.shape[1], out_width, page, _stream(tables),
-        ),
-        "vrh_sequence_metadata",
-    )
+    with torch.cuda.device(device):
+        lib.check(
+            lib.vrh_sequence_metadata(
+                tables.data_ptr(), tables.shape[0], tables.stride(0), table_rows.data_ptr(),
+                context_lengths.data_ptr(), query_lengths.data_ptr(), wide[0].data_ptr(),
+                wide[1].data_ptr(), wide[2].data_ptr(), mask.data_ptr(), block_tables.data_ptr(),
+                out_width, lengths.data_ptr(), cu.data_ptr(), n, tokens, tables.shape[1],
+                out_width, page, _stream(tables),
+            ),
+            "vrh_sequence_metadata",
+        )
     return wide[0], wide[1], wide[2], mask, block_tables, lengths, cu

@@ -19,6 +19,7 @@ from __future__ import annotations
 
 import torch
 
+from vllm_rlt.kernels._extension import plain_calls
 from vllm_rlt.kernels._hip import library
 from vllm_rlt.kernels.hip_attention import _check_int, _on_gpu, dtype_code
 
@@ -120,6 +121,10 @@ def kv_append_q8(key_cache, value_cache, scales, k, v, block_tables, context_len
     older tokens are rounded to it; any other block starts with the scale its new tokens need.
     A block that is written belongs to one of the sequences: shared blocks are copied first.
     """
+    plain = plain_calls()
+    if plain is not None and plain.append_q8(key_cache, value_cache, scales, k, v, block_tables,
+                                             context_lengths, cu_seqlens_q):
+        return
     _check_cache_q8(key_cache, value_cache, scales)
     device = key_cache.device
     for name, rows in (("k", k), ("v", v)):
@@ -152,6 +157,11 @@ def kv_append_q8(key_cache, value_cache, scales, k, v, block_tables, context_len
 def kv_read_q8(key_cache, value_cache, scales, pages, dtype=torch.bfloat16):
     """The values that ``pages`` (int64 block ids) stand for, rounded to ``dtype``: K and V
     ``[len(pages), block_size, kv_heads, head_dim]``. Ids outside the pool read as zeros."""
+    plain = plain_calls()
+    if plain is not None:
+        read = plain.read_q8(key_cache, value_cache, scales, pages, dtype)
+        if read is not None:
+            return read
     _check_cache_q8(key_cache, value_cache, scales)
     code = dtype_code(dtype)
     device = key_cache.device
@@ -176,6 +186,12 @@ def paged_attention_q8(q, key_cache, value_cache, scales, block_tables, context_
     ``window`` > 0 keeps the last ``window`` keys. Rows of length 0 give zeros."""
     if type(window) is not int or not 0 <= window < 1 << 31:
         raise ValueError("window must be a nonnegative integer")
+    plain = plain_calls()
+    if plain is not None and out is None:
+        output = plain.decode_q8(q, key_cache, value_cache, scales, block_tables, context_lengths,
+                                 window)
+        if output is not None:
+            return output
     q, out = _check_queries(q, key_cache, value_cache, scales, out)
     context_lengths = _check_tables(block_tables, context_lengths, q.device)
     rows = q.shape[0]
@@ -206,6 +222,12 @@ def paged_prefill_attention_q8(q, key_cache, value_cache, scales, block_tables, 
     ``paged_prefill_attention`` with ``scales``. Rows of ``out`` that belong to no sequence are
     not written. With ``max_seqlen_q`` <= 8 every query equals its single-query decode bit for
     bit."""
+    plain = plain_calls()
+    if plain is not None and out is None:
+        output = plain.prefill_q8(q, key_cache, value_cache, scales, block_tables, context_lengths,
+                                  cu_seqlens_q, max_seqlen_q)
+        if output is not None:
+            return output
     q, out = _check_queries(q, key_cache, value_cache, scales, out)
     context_lengths = _check_tables(block_tables, context_lengths, q.device)
     sequences = block_tables.shape[0]
