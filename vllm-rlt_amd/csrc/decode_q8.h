@@ -41,6 +41,10 @@ struct DecodeQ8Args {
   int32_t slots;  // most splits of a row
   int32_t tiles;  // waves of up to 16 q heads per KV head (MFMA kernel)
   int32_t units;  // kv_heads * tiles
+  int32_t compact;  // waves share the splits that exist (MFMA kernel)
+  int32_t split_unit;  // splits are whole multiples of this many pages (a power of two)
+  int32_t min_shift;   // log2 of d.min_bps, a short row's pages per split, or -1
+  int32_t long_shift;  // log2 of d.long_bps, a longer row's, or -1
 };
 
 // A page id brought into the pool: an id that is not one of its blocks (a caller's
@@ -141,6 +145,15 @@ __device__ __forceinline__ void v_scale(int e, float& vs, float& ps) {
     vs = q8_scale(e);
     ps = 1.f;
   }
+}
+
+// The LDS-direct loads of common.h for bytes that are read once (see lds_dma16).
+__device__ __forceinline__ void lds_stream16(const void* g, uint32_t m0) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, off nt" ::"v"(g), "{m0}"(m0) : "memory");
+}
+__device__ __forceinline__ void lds_stream16_s(const void* base, uint32_t lane_off, uint32_t m0) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(lane_off), "s"(base), "{m0}"(m0)
+               : "memory");
 }
 
 // 16 bytes at an LDS byte offset.

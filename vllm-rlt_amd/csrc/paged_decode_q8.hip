@@ -15,9 +15,15 @@
 namespace vrh {
 namespace {
 
-// Tokens of the shortest split, and the most splits of a row.
+// Splits of rows of up to kShortTokens visible tokens and of longer ones, and the most
+// splits of a row. Long rows come in batches or are cut into many splits anyway, and a
+// split costs a wave's start and a partial: 64 rows of 512-4096 tokens (16 x 128 heads)
+// 113 us with splits of 128 tokens throughout, 107 with 256; 512 no better. Short rows
+// are what few waves have: one row of 300 tokens in three splits.
 constexpr int kSplitTokens = 128;
-constexpr int kMaxSplitsQ8 = 32;
+constexpr int kLongTokens = 256;
+constexpr int kShortTokens = 2048;
+constexpr int kMaxSplitsQ8 = 64;  // a lane each in the merge
 
 struct PartitionQ8 {
   int start;   // first visible token
@@ -37,8 +43,23 @@ __device__ __forceinline__ PartitionQ8 partition_q8(int n, const DecodeQ8Args& a
     p.first = p.start / a.d.block_size;
     p.pages = (n - 1) / a.d.block_size + 1 - p.first;
   }
-  p.bps = max(a.d.min_bps, ceil_div(p.pages, a.slots));
-  p.nsplit = ceil_div(p.pages, p.bps);
+  // Fewer slots than the most splits: the table (or window) has no longer rows, or one
+  // split is asked for.
+  if (a.slots == 1) {
+    p.bps = (p.pages + a.split_unit - 1) & -a.split_unit;
+    p.nsplit = 1;
+  } else {
+    const bool longer = p.pages > a.d.short_pages;
+    const int shift = longer ? a.long_shift : a.min_shift;
+    if (shift >= 0 && p.pages <= kMaxSplitsQ8 << shift) {
+      p.bps = 1 << shift;  // (no division: a wave does this before its first load)
+      p.nsplit = (p.pages + p.bps - 1) >> shift;
+    } else {
+      p.bps = max(longer ? a.d.long_bps : a.d.min_bps, (p.pages + kMaxSplitsQ8 - 1) / kMaxSplitsQ8);
+      p.bps = (p.bps + a.split_unit - 1) & -a.split_unit;
+      p.nsplit = (int)((uint32_t)(p.pages + p.bps - 1) / (uint32_t)p.bps);
+    }
+  }
   return p;
 }
 
@@ -46,12 +67,118 @@ __device__ __forceinline__ int page_of(int pos, const DecodeQ8Args& a) {
   return a.d.bs_shift >= 0 ? pos >> a.d.bs_shift : pos / a.d.block_size;
 }
 
-// The (row, split) of a workgroup: item blockIdx.x / units, split-major within a row,
-// rows in order.
-__device__ __forceinline__ bool q8_item(const DecodeQ8Args& a, int64_t& row, int& split) {
-  const int64_t item = blockIdx.x / a.units;
-  row = a.d.row_base + item / a.slots;
-  split = (int)(item - (item / a.slots) * a.slots);
+// Sum over the lanes up to this one.
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, true);  // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, true);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // row_bcast:15
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // row_bcast:31
+  return x;
+}
+
+// Work of the matrix kernel's waves. For up to kCompactRows rows the splits that exist
+// are numbered (rows in order), and a KV head's waves take equal shares of consecutive
+// ones: one split each while there are no more than kRounds times as many as waves are
+// resident, else runs of a row's splits (within kSegment pages). Which wave takes a split
+// changes no result, since each split has its own state. So no wave without work holds
+// the LDS that another waits for, however wide the tables are (48 decode rows of a mixed
+// step under tables of 512 pages: 119 us with a wave for each slot, 85). One share per
+// resident wave, no starts but the first, was slower (64 rows 117 us against 107): the
+// heads of a block, neighbours in memory, drift apart. Each wave counts the rows' splits
+// itself, 64 rows at a time; beyond kCompactRows a wave takes one split, workgroups being
+// dealt slots x rows.
+constexpr int kRounds = 8;
+constexpr int kCompactRows = 512;
+constexpr int kSegment = 64;
+
+struct ItemQ8 {
+  int64_t row;   // work row
+  int64_t trow;  // table row
+  int64_t qrow;  // query and output row
+  int n;         // visible length
+  int split, splits;  // first split, and how many
+};
+
+// A lane's row of up to 64 consecutive ones: its splits, and the most of them in a run.
+struct RowQ8 {
+  int64_t trow, qrow;
+  int n, splits, most;
+};
+__device__ __forceinline__ RowQ8 q8_row(const DecodeQ8Args& a, int64_t row) {
+  RowQ8 r = {0, 0, -1, 0, 1};
+  if (row < a.d.rows) r.n = row_length(row, a.d, &r.trow, &r.qrow);
+  if (r.n > 0) {
+    const PartitionQ8 P = partition_q8(r.n, a);
+    r.splits = P.nsplit;
+    r.most = (P.bps & (P.bps - 1)) == 0 ? kSegment >> (31 - __builtin_clz(P.bps)) : kSegment / P.bps;
+    r.most = max(1, r.most);
+  } else if (r.n == 0) {
+    r.splits = 1;
+  }
+  return r;
+}
+
+// A wave's share of a KV head's splits, all of it wave-uniform but `r` and `upto`.
+struct ShareQ8 {
+  RowQ8 r;          // this lane's row of the 64 from `base` on
+  int upto;         // splits of those rows up to this lane's
+  int64_t base;
+  uint32_t before;  // splits of the rows before `base`
+  uint32_t next, end;
+};
+
+__device__ __forceinline__ void q8_share(const DecodeQ8Args& a, uint32_t wave, uint32_t waves, ShareQ8& s) {
+  const int lane = threadIdx.x & 63;
+  if (a.compact == 0) {
+    s.next = wave;
+    s.end = wave + 1;
+    return;
+  }
+  s.base = 0;
+  s.before = 0;
+  s.r = q8_row(a, lane);
+  s.upto = wave_scan(s.r.splits);
+  uint32_t total = (uint32_t)__builtin_amdgcn_readlane(s.upto, 63);
+  for (int64_t base = 64; base < a.d.rows; base += 64)
+    total += (uint32_t)wave_sum_i(q8_row(a, base + lane).splits);
+  s.next = (uint32_t)((uint64_t)wave * total / waves);
+  s.end = (uint32_t)((uint64_t)(wave + 1) * total / waves);
+}
+
+// The share's next run; false when it is done.
+__device__ __forceinline__ bool q8_next(const DecodeQ8Args& a, ShareQ8& s, ItemQ8& it) {
+  if (s.next >= s.end) return false;
+  if (a.compact == 0) {
+    it.row = a.d.row_base + s.next / (uint32_t)a.slots;
+    it.split = (int)(s.next % (uint32_t)a.slots);
+    it.splits = 1;
+    it.n = row_length(it.row, a.d, &it.trow, &it.qrow);
+    ++s.next;
+    return true;
+  }
+  for (;;) {
+    const uint32_t all = (uint32_t)__builtin_amdgcn_readlane(s.upto, 63);
+    if (s.next - s.before < all) break;
+    s.before += all;
+    s.base += 64;
+    s.r = q8_row(a, s.base + (threadIdx.x & 63));
+    s.upto = wave_scan(s.r.splits);
+  }
+  // First lane whose splits end past the next one.
+  const uint32_t at = s.next - s.before;
+  const int pick = __builtin_ffsll((long long)__ballot((uint32_t)s.upto > at)) - 1;
+  it.row = s.base + pick;
+  it.trow = ((int64_t)__builtin_amdgcn_readlane((int)(s.r.trow >> 32), pick) << 32) |
+            (uint32_t)__builtin_amdgcn_readlane((int)s.r.trow, pick);
+  it.qrow = ((int64_t)__builtin_amdgcn_readlane((int)(s.r.qrow >> 32), pick) << 32) |
+            (uint32_t)__builtin_amdgcn_readlane((int)s.r.qrow, pick);
+  it.n = __builtin_amdgcn_readlane(s.r.n, pick);
+  const int splits = __builtin_amdgcn_readlane(s.r.splits, pick);
+  it.split = (int)at - (__builtin_amdgcn_readlane(s.upto, pick) - splits);
+  it.splits = min(min(__builtin_amdgcn_readlane(s.r.most, pick), splits - it.split), (int)(s.end - s.next));
+  s.next += (uint32_t)it.splits;
   return true;
 }
 
@@ -216,11 +343,13 @@ __global__ __launch_bounds__(64) void paged_decode_q8_kernel(DecodeQ8Args a) {
 }
 
 // ------------------------------------------------ 16-bit queries on MFMA
-// One wave per (split, KV head, row) serves up to 16 q heads of the KV head (the
+// One wave per (run of splits, KV head, row) serves up to 16 q heads of the KV head (the
 // columns of v_mfma_f32_16x16x32; groups of more take several waves):
 //  * K and V come in chunks of 32 tokens straight into a ring of kStages wave-private
-//    LDS stages, kStages - 1 chunks ahead: no registers are held by loads in flight and
-//    no barrier is needed. One load instruction covers RPI whole rows of one page.
+//    LDS stages, kStages - 1 chunks ahead and across the splits of the run: no registers
+//    are held by loads in flight and no barrier is needed. One load instruction covers
+//    RPI whole rows; the block size is a power of two of at least 16, so 16-token steps
+//    lie in one page and take one (scalar) address.
 //  * S^T = K Q^T per 16 tokens: bytes are converted to the query's type (exact), 16 a
 //    lane per LDS read, which is two k-steps; the dims of Q^T's k-slots follow that
 //    order. The page's K scale joins the softmax scale on the fp32 scores.
@@ -262,260 +391,310 @@ __device__ __forceinline__ void lds_dma4(const void* g, uint32_t m0) {
   asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(g), "{m0}"(m0) : "memory");
 }
 
+__device__ __forceinline__ float readlane_f32(float x, int lane) {
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane));
+}
+
 template <typename T, int D>
 __global__ __launch_bounds__(64) void paged_decode_q8_mfma_kernel(DecodeQ8Args a) {
   constexpr int KCH = D / 16;        // 16-byte chunks per row
-  constexpr int RPI = 64 / KCH;      // rows per load instruction
-  constexpr int NI = kChunk / RPI;   // load instructions per chunk, K and V each
+  constexpr int RPI = 64 / KCH;      // rows per load instruction (8 or 16)
+  constexpr int IPS = 16 / RPI;      // load instructions per 16-token step
+  constexpr int NI = 2 * IPS;        // per chunk, K and V each
   constexpr int KC = D / 64;         // LDS reads per 16 tokens of K
   constexpr int DT = D / 16;         // 16-dim tiles of O^T
   constexpr int kStage = 2 * kChunk * D;
-  __shared__ __attribute__((aligned(256))) uint8_t stage[kStages * kStage + 256];
+  constexpr bool kF16 = std::is_same<T, f16_t>::value;
+  __shared__ __attribute__((aligned(256))) uint8_t stage[kStages * kStage + 4 * kSegment];
   const int lane = threadIdx.x;
   const int col = lane & 15, grp = lane >> 4;
+  const int bs = a.d.block_size, sh = a.d.bs_shift;
 
-  int64_t row;
-  int split;
-  if (!q8_item(a, row, split)) return;
-  const int unit = (int)(blockIdx.x % a.units);
-  const int kvh = unit / a.tiles;
+  const uint32_t share = blockIdx.x / (uint32_t)a.units;
+  const int unit = (int)(blockIdx.x - share * (uint32_t)a.units);
+  const int kvh = a.tiles == 1 ? unit : unit / a.tiles;
   const int head0 = kvh * a.d.group + (unit - kvh * a.tiles) * 16;
   const int heads = min(16, (kvh + 1) * a.d.group - head0);
-  int64_t trow, qrow;
-  const int n = row_length(row, a.d, &trow, &qrow);
-  if (n < 0) return;
   const bool hcol = col < heads;
-  T* out = reinterpret_cast<T*>(a.d.out) + qrow * a.d.o_row + (int64_t)(head0 + col) * a.d.o_head + 4 * grp;
-  if (n == 0) {
-    if (split == 0 && hcol) {
-#pragma unroll
-      for (int t = 0; t < DT; ++t) *reinterpret_cast<u32x2_t*>(out + 16 * t) = u32x2_t{0u, 0u};
-    }
-    return;
-  }
-  const PartitionQ8 P = partition_q8(n, a);
-  if (split >= P.nsplit) return;
-  const int bs = a.d.block_size;
-  const int s0 = P.first + split * P.bps, s1 = min(s0 + P.bps, P.first + P.pages);
-  const int32_t* table = a.d.tables + trow * a.d.table_stride;
-
-  // Q^T operands of k-step (c, i): dims 64 c + 16 grp + 8 i .. + 7.
-  u32x4_t qop[KC][2];
-  {
-    const T* qp = reinterpret_cast<const T*>(a.d.q) + qrow * a.d.q_row +
-                  (int64_t)(head0 + (hcol ? col : 0)) * a.d.q_head + 16 * grp;
-#pragma unroll
-    for (int c = 0; c < KC; ++c)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const u32x4_t x = *reinterpret_cast<const u32x4_t*>(qp + 64 * c + 8 * i);
-        qop[c][i] = hcol ? x : u32x4_t{0u, 0u, 0u, 0u};
-      }
-  }
   const uint8_t* kbase = reinterpret_cast<const uint8_t*>(a.d.k) + (int64_t)kvh * a.d.k_head;
   const uint8_t* vbase = reinterpret_cast<const uint8_t*>(a.d.v) + (int64_t)kvh * a.d.v_head;
   const uint8_t* sbase = a.scales + (int64_t)kvh * a.s_head;
   const uint32_t lds0 = lds_offset(stage);
   const uint32_t lds_sc = lds0 + kStages * kStage;
 
-  // This lane's byte offset within a load instruction's rows; instructions whose rows
-  // have the swizzle's top bit flipped take the second.
+  // This lane's byte offset of load instruction r of a chunk from its 16-token step's
+  // first row: row RPI r + lane / KCH of the chunk, chunk by the row's swizzle.
   const int lrow = lane / KCH;
-  uint32_t loff[2];
+  uint32_t loff[NI];
 #pragma unroll
-  for (int x = 0; x < 2; ++x)
-    loff[x] = (uint32_t)lrow * (uint32_t)a.d.k_token +
-              16 * ((lane % KCH) ^ q8_swizzle<D>(lrow) ^ (x * KCH / 2));
-  auto flip = [](int r) { return D == 128 ? (r ^ (r >> 1)) & 1 : r & 1; };
+  for (int r = 0; r < NI; ++r)
+    loff[r] = (uint32_t)((RPI * r + lrow) & 15) * (uint32_t)a.d.k_token +
+              16 * ((lane % KCH) ^ q8_swizzle<D>(RPI * r + lrow));
   // LDS byte offsets of the operand reads.
-  uint32_t koff[2];
+  uint32_t koff[2][KC], voff[DT];
 #pragma unroll
-  for (int t = 0; t < 2; ++t) koff[t] = lds0 + (16 * t + col) * D + 16 * (grp ^ q8_swizzle<D>(16 * t + col));
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int c = 0; c < KC; ++c)
+      koff[t][c] = lds0 + (16 * t + col) * D + ((16 * (grp ^ q8_swizzle<D>(16 * t + col))) ^ (64 * c));
   const int vrow = (col >> 1) < 4 ? 4 * grp + (col >> 1) : 12 + 4 * grp + (col >> 1);
-  const uint32_t voff = lds0 + kChunk * D + vrow * D + 16 * q8_swizzle<D>(vrow) + 8 * (col & 1);
+#pragma unroll
+  for (int t = 0; t < DT; ++t)
+    voff[t] = lds0 + kChunk * D + vrow * D + ((16 * q8_swizzle<D>(vrow)) ^ (16 * t)) + 8 * (col & 1);
 
-  float m = -1e30f, lsum = 0.f;  // of this lane's head column; lsum over its token slots
-  f32x4_t acc[DT];
+  ShareQ8 mine;
+  q8_share(a, share, gridDim.x / (uint32_t)a.units, mine);
+  ItemQ8 it;
+  while (q8_next(a, mine, it)) {
+    const int n = it.n;
+    T* out = reinterpret_cast<T*>(a.d.out) + it.qrow * a.d.o_row + (int64_t)(head0 + col) * a.d.o_head + 4 * grp;
+    if (n <= 0) {
+      if (n == 0 && it.split == 0 && hcol) {
 #pragma unroll
-  for (int t = 0; t < DT; ++t) acc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-
-  for (int seg = s0; seg < s1; seg += 64) {
-    const int seg1 = min(s1, seg + 64);
-    const int blk = seg + lane < seg1 ? pool_block(table[seg + lane], a) : 0;
-    // The pages' exponents: the aligned word around each pair, and which half it is.
-    const uint8_t* sp = sbase + (int64_t)blk * a.s_block;
-    const uint64_t high = __ballot(((uintptr_t)sp & 2) != 0);
-    lds_dma4((const void*)((uintptr_t)sp & ~(uintptr_t)3), __builtin_amdgcn_readfirstlane(lds_sc));
-    const int t0 = seg * bs;  // first token of the segment
-    const int tb = max(P.start, t0);
-    const int te = (int)min((int64_t)n, (int64_t)seg1 * bs);
-    // Chunks start at the 16-token step of the page that the first token is in.
-    const int c0 = t0 + ((tb - t0) & ~15);
-    const int chunks = (te - c0 + kChunk - 1) / kChunk;
-
-    auto load = [&](int j, auto st_c) {
-      constexpr int st = decltype(st_c)::value;
-      const int p0 = c0 + j * kChunk;
-      const uint32_t kl = lds0 + st * kStage, vl = kl + kChunk * D;
-      if (p0 >= tb && te - p0 >= kChunk) {
-        int page = (int)__builtin_amdgcn_readfirstlane(page_of(p0, a) - seg);
-        int off = p0 - (seg + page) * bs;
-#pragma unroll
-        for (int r = 0; r < NI; ++r) {
-          const uint32_t b = __builtin_amdgcn_readlane(blk, page);
-          const uint64_t at = (uint64_t)b * (uint64_t)a.d.k_block + (uint64_t)((uint32_t)off * (uint64_t)(uint32_t)a.d.k_token);
-          lds_dma16_s(kbase + at, loff[flip(r)], __builtin_amdgcn_readfirstlane(kl + 1024 * r));
-          lds_dma16_s(vbase + at, loff[flip(r)], __builtin_amdgcn_readfirstlane(vl + 1024 * r));
-          off += RPI;
-          if (off >= bs) {
-            off -= bs;
-            ++page;
-          }
-        }
-        return;
+        for (int t = 0; t < DT; ++t) *reinterpret_cast<u32x2_t*>(out + 16 * t) = u32x2_t{0u, 0u};
       }
-      // A chunk that reaches outside the visible tokens reads the nearest visible one
-      // there: masked out of the softmax, and as finite as the row itself.
-#pragma unroll
-      for (int r = 0; r < NI; ++r) {
-        const int i = RPI * r + lrow;
-        const int pos = max(tb, te - p0 > i ? p0 + i : te - 1);
-        const int page = page_of(pos, a) - seg;
-        const int off = pos - (seg + page) * bs;
-        const int64_t at = (int64_t)shfl_i32(blk, page) * a.d.k_block + (int64_t)off * a.d.k_token +
-                           16 * ((lane % KCH) ^ q8_swizzle<D>(i));
-        lds_dma16(kbase + at, __builtin_amdgcn_readfirstlane(kl + 1024 * r));
-        lds_dma16(vbase + at, __builtin_amdgcn_readfirstlane(vl + 1024 * r));
-      }
-    };
-    auto attend = [&](int j, auto st_c) {
-      constexpr int st = decltype(st_c)::value;
-      const int p0 = c0 + j * kChunk;
-      // Scales of the chunk's two 16-token tiles.
-      float ks[2], vs[2], ps[2];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        const int pos = min(max(p0 + 16 * t, tb), te - 1);
-        const int page = __builtin_amdgcn_readfirstlane(page_of(pos, a) - seg);
-        const uint32_t w = __builtin_amdgcn_readfirstlane(
-            *reinterpret_cast<const uint32_t*>(stage + kStages * kStage + 4 * page));
-        const uint32_t e = w >> ((high >> page & 1) ? 16 : 0);
-        ks[t] = q8_scale(e & 255) * a.d.scale_log2;
-        v_scale<T>(e >> 8 & 255, vs[t], ps[t]);
-      }
-      f32x4_t sc[2];
-#pragma unroll
-      for (int t = 0; t < 2; ++t) {
-        sc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < KC; ++c) {
-          const u32x4_t x = lds_read16((koff[t] ^ (64 * c)) + st * kStage);
-          sc[t] = MfmaQ8<T>::run(MfmaQ8<T>::widen(x[0], x[1], 1.f, 1.f), qop[c][0], sc[t]);
-          sc[t] = MfmaQ8<T>::run(MfmaQ8<T>::widen(x[2], x[3], 1.f, 1.f), qop[c][1], sc[t]);
-        }
-      }
-      float mx = -INFINITY;
-      if (p0 >= tb && te - p0 >= kChunk) {
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            sc[t][i] *= ks[t];
-            mx = fmaxf(mx, sc[t][i]);
-          }
-      } else {
-        const int lo = tb - p0 - 4 * grp, hi = te - p0 - 4 * grp;
-#pragma unroll
-        for (int t = 0; t < 2; ++t)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            sc[t][i] = 16 * t + i >= lo && 16 * t + i < hi ? sc[t][i] * ks[t] : -INFINITY;
-            mx = fmaxf(mx, sc[t][i]);
-          }
-      }
-      // Over the four lane groups of the head column.
-      {
-        const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-        mx = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
-        const auto y = __builtin_amdgcn_permlane16_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-        mx = fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
-      }
-      // The reference moves only when a score passes it by more than kSlack, so that most
-      // chunks leave the accumulators alone.
-      if (__any(mx > m + Weights<T>::kSlack)) {
-        const float top = fmaxf(m, mx - Weights<T>::kLift);
-        const float corr = fast_exp2(m - top);
-        lsum *= corr;
-#pragma unroll
-        for (int t = 0; t < DT; ++t) acc[t] *= corr;
-        m = top;
-      }
-      float p[2][4];
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          p[t][i] = fast_exp2(sc[t][i] - m);
-          lsum += p[t][i];
-          if constexpr (std::is_same<T, f16_t>::value) p[t][i] *= ps[t];
-        }
-      const u32x4_t pop = u32x4_t{pack2<T>(p[0][0], p[0][1]), pack2<T>(p[0][2], p[0][3]),
-                                  pack2<T>(p[1][0], p[1][1]), pack2<T>(p[1][2], p[1][3])};
-#pragma unroll
-      for (int t = 0; t < DT; ++t) {
-        const u32x2_t x = lds_tr8((voff ^ (16 * t)) + st * kStage);
-        acc[t] = MfmaQ8<T>::run(MfmaQ8<T>::widen(x[0], x[1], vs[0], vs[1]), pop, acc[t]);
-      }
-    };
-    using S0 = std::integral_constant<int, 0>;
-    using S1 = std::integral_constant<int, 1>;
-    using S2 = std::integral_constant<int, 2>;
-    static_assert(kStages == 3, "the steps below");
-    load(0, S0{});
-    if (chunks > 1) load(1, S1{});
-    // Step j: chunk j has landed (only the loads of j + 1 may be in flight); the stage of
-    // j - 1, whose reads have returned, takes chunk j + 2.
-    auto step = [&](int j, auto now, auto next) {
-      if (j + 1 < chunks) wait_loads<2 * NI>();
-      else wait_loads<0>();
-      if (j + 2 < chunks) load(j + 2, next);
-      attend(j, now);
-      wait_lds();
-    };
-    for (int j = 0; j < chunks; j += 3) {
-      step(j, S0{}, S2{});
-      if (j + 1 >= chunks) break;
-      step(j + 1, S1{}, S0{});
-      if (j + 2 >= chunks) break;
-      step(j + 2, S2{}, S1{});
+      continue;
     }
-  }
-  lsum += shfl_xor_f32(lsum, 16);
-  lsum += shfl_xor_f32(lsum, 32);
-  if (!hcol) return;
-  if (P.nsplit == 1) {
-    const float inv = 1.f / lsum;
+    const PartitionQ8 P = partition_q8(n, a);
+    if (it.split >= P.nsplit) continue;
+    const int s0 = P.first + it.split * P.bps;
+    const int s1 = min(s0 + it.splits * P.bps, P.first + P.pages);
+    const int32_t* table = a.d.tables + it.trow * a.d.table_stride;
+    // The first page ids travel with the queries.
+    int ids = s0 + lane < min(s1, s0 + kSegment) ? table[s0 + lane] : 0;
+
+    // Q^T operands of k-step (c, i): dims 64 c + 16 grp + 8 i .. + 7.
+    u32x4_t qop[KC][2];
+    {
+      const T* qp = reinterpret_cast<const T*>(a.d.q) + it.qrow * a.d.q_row +
+                    (int64_t)(head0 + (hcol ? col : 0)) * a.d.q_head + 16 * grp;
 #pragma unroll
-    for (int t = 0; t < DT; ++t)
-      *reinterpret_cast<u32x2_t*>(out + 16 * t) =
-          u32x2_t{pack2<T>(acc[t][0] * inv, acc[t][1] * inv), pack2<T>(acc[t][2] * inv, acc[t][3] * inv)};
-    return;
-  }
-  const int64_t idx = (row * a.d.q_heads + head0 + col) * a.slots + split;
-  if (grp == 0) {
-    a.d.part_ml[idx * 2] = m;
-    a.d.part_ml[idx * 2 + 1] = lsum;
-  }
-  float* dst = a.d.part_acc + idx * D + 4 * grp;
+      for (int c = 0; c < KC; ++c)
 #pragma unroll
-  for (int t = 0; t < DT; ++t) *reinterpret_cast<f32x4_t*>(dst + 16 * t) = acc[t];
+        for (int i = 0; i < 2; ++i) {
+          const u32x4_t x = *reinterpret_cast<const u32x4_t*>(qp + 64 * c + 8 * i);
+          qop[c][i] = hcol ? x : u32x4_t{0u, 0u, 0u, 0u};
+        }
+    }
+
+    float m = -1e30f, lsum = 0.f;  // of this lane's head column; lsum over its token slots
+    f32x4_t acc[DT];
+#pragma unroll
+    for (int t = 0; t < DT; ++t) acc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    int split = it.split;
+    // The end of a split: its partial (or the row's output), and a fresh state.
+    auto flush = [&]() __attribute__((always_inline)) {
+      lsum += shfl_xor_f32(lsum, 16);
+      lsum += shfl_xor_f32(lsum, 32);
+      if (hcol && P.nsplit == 1) {
+        const float inv = 1.f / lsum;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+          *reinterpret_cast<u32x2_t*>(out + 16 * t) =
+              u32x2_t{pack2<T>(acc[t][0] * inv, acc[t][1] * inv), pack2<T>(acc[t][2] * inv, acc[t][3] * inv)};
+      } else if (hcol) {
+        const int64_t idx = (it.row * a.d.q_heads + head0 + col) * a.slots + split;
+        if (grp == 0) {
+          a.d.part_ml[idx * 2] = m;
+          a.d.part_ml[idx * 2 + 1] = lsum;
+        }
+        float* dst = a.d.part_acc + idx * D + 4 * grp;
+#pragma unroll
+        for (int t = 0; t < DT; ++t) *reinterpret_cast<f32x4_t*>(dst + 16 * t) = acc[t];
+      }
+      ++split;
+      m = -1e30f;
+      lsum = 0.f;
+#pragma unroll
+      for (int t = 0; t < DT; ++t) acc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    };
+
+    for (int seg = s0; seg < s1; seg += kSegment) {
+      const int seg1 = min(s1, seg + kSegment);
+      if (seg > s0) ids = seg + lane < seg1 ? table[seg + lane] : 0;
+      const int blk = pool_block(ids, a);
+      // The pages' exponents: the aligned word around each pair.
+      const uint8_t* sp = sbase + (int64_t)blk * a.s_block;
+      lds_dma4((const void*)((uintptr_t)sp & ~(uintptr_t)3), __builtin_amdgcn_readfirstlane(lds_sc));
+      const uint64_t at = (uint64_t)(uint32_t)blk * (uint64_t)a.d.k_block;
+      const int at_lo = (int)at, at_hi = (int)(at >> 32);
+      const int t0 = seg << sh;  // first token of the segment
+      const int tb = max(P.start, t0);
+      const int te = (int)min((int64_t)n, (int64_t)seg1 << sh);
+      // Chunk j holds tokens t0 + 32 j ..; those before the window's are not read.
+      const int j0 = (tb - t0) / kChunk, j1 = (te - t0 + kChunk - 1) / kChunk;
+      // Chunks per split (one split longer than a segment is flushed after the last).
+      const int per = P.bps > kSegment ? INT32_MAX : (P.bps << sh) / kChunk;
+
+      auto load = [&](int j, auto st_c) __attribute__((always_inline)) {
+        constexpr int st = decltype(st_c)::value;
+        const int p0 = j * kChunk;  // from t0
+        const uint32_t kl = lds0 + st * kStage, vl = kl + kChunk * D;
+        if (t0 + p0 >= tb && te - t0 - p0 >= kChunk) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int page = (p0 + 16 * h) >> sh;
+            const uint32_t row = (uint32_t)(p0 + 16 * h) & (uint32_t)(bs - 1);
+            const uint64_t off = ((uint64_t)(uint32_t)__builtin_amdgcn_readlane(at_hi, page) << 32 |
+                                  (uint32_t)__builtin_amdgcn_readlane(at_lo, page)) +
+                                 (uint64_t)row * (uint32_t)a.d.k_token;
+#pragma unroll
+            for (int i = 0; i < IPS; ++i) {
+              const int r = IPS * h + i;
+              lds_stream16_s(kbase + off, loff[r], __builtin_amdgcn_readfirstlane(kl + 1024 * r));
+              lds_stream16_s(vbase + off, loff[r], __builtin_amdgcn_readfirstlane(vl + 1024 * r));
+            }
+          }
+          return;
+        }
+        // A chunk that reaches outside the visible tokens reads the nearest visible one
+        // there: masked out of the softmax, and as finite as the row itself.
+#pragma unroll 1
+        for (int r = 0; r < NI; ++r) {
+          const int i = RPI * r + lrow;
+          const int pos = min(max(p0 + i, tb - t0), te - t0 - 1);
+          const int64_t off = (int64_t)shfl_i32(blk, pos >> sh) * a.d.k_block +
+                              (int64_t)(pos & (bs - 1)) * a.d.k_token +
+                              16 * ((lane % KCH) ^ q8_swizzle<D>(i));
+          lds_stream16(kbase + off, __builtin_amdgcn_readfirstlane(kl + 1024 * r));
+          lds_stream16(vbase + off, __builtin_amdgcn_readfirstlane(vl + 1024 * r));
+        }
+      };
+      // One page a lane, set when the exponents have landed: the factor of its scores,
+      // and its V scale.
+      float kf = 0.f, vf = 0.f, pf = 1.f;
+      auto scales = [&]() {
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(stage + kStages * kStage + 4 * lane);
+        const uint32_t e = ((uintptr_t)sp & 2) ? w >> 16 : w;
+        // (0, of a page never written, would make NaN of masked scores)
+        kf = q8_scale(max((int)(e & 255), kLeastExponent)) * a.d.scale_log2;
+        v_scale<T>(e >> 8 & 255, vf, pf);
+      };
+      auto attend = [&](int j, auto st_c) __attribute__((always_inline)) {
+        constexpr int st = decltype(st_c)::value;
+        const int p0 = j * kChunk;
+        f32x4_t sc[2];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          sc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < KC; ++c) {
+            const u32x4_t x = lds_read16(koff[t][c] + st * kStage);
+            sc[t] = MfmaQ8<T>::run(MfmaQ8<T>::widen(x[0], x[1], 1.f, 1.f), qop[c][0], sc[t]);
+            sc[t] = MfmaQ8<T>::run(MfmaQ8<T>::widen(x[2], x[3], 1.f, 1.f), qop[c][1], sc[t]);
+          }
+        }
+        // Scales of the chunk's two 16-token tiles (the second may lie past the last page).
+        const int g0 = min(p0, te - t0 - 1) >> sh, g1 = min(p0 + 16, te - t0 - 1) >> sh;
+        const float ks[2] = {readlane_f32(kf, g0), readlane_f32(kf, g1)};
+        const float vs[2] = {readlane_f32(vf, g0), readlane_f32(vf, g1)};
+        if (!(t0 + p0 >= tb && te - t0 - p0 >= kChunk)) {
+          const int lo = tb - t0 - p0 - 4 * grp, hi = te - t0 - p0 - 4 * grp;
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              sc[t][i] = 16 * t + i >= lo && 16 * t + i < hi ? sc[t][i] : -INFINITY;
+        }
+        float mx = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])) * ks[0],
+                         fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])) * ks[1]);
+        // Over the four lane groups of the head column.
+        {
+          const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+          mx = fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1]));
+          const auto y = __builtin_amdgcn_permlane16_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+          mx = fmaxf(__uint_as_float(y[0]), __uint_as_float(y[1]));
+        }
+        // The reference moves only when a score passes it by more than kSlack, so that most
+        // chunks leave the accumulators alone.
+        if (__any(mx > m + Weights<T>::kSlack)) {
+          const float top = fmaxf(m, mx - Weights<T>::kLift);
+          const float corr = fast_exp2(m - top);
+          lsum *= corr;
+#pragma unroll
+          for (int t = 0; t < DT; ++t) acc[t] *= corr;
+          m = top;
+        }
+        float p[2][4];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) p[t][i] = fast_exp2(fmaf(sc[t][i], ks[t], -m));
+        lsum += ((p[0][0] + p[0][1]) + (p[0][2] + p[0][3])) + ((p[1][0] + p[1][1]) + (p[1][2] + p[1][3]));
+        if constexpr (kF16) {
+          const float ps[2] = {readlane_f32(pf, g0), readlane_f32(pf, g1)};
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) p[t][i] *= ps[t];
+        }
+        const u32x4_t pop = u32x4_t{pack2<T>(p[0][0], p[0][1]), pack2<T>(p[0][2], p[0][3]),
+                                    pack2<T>(p[1][0], p[1][1]), pack2<T>(p[1][2], p[1][3])};
+#pragma unroll
+        for (int t = 0; t < DT; ++t) {
+          const u32x2_t x = lds_tr8(voff[t] + st * kStage);
+          acc[t] = MfmaQ8<T>::run(MfmaQ8<T>::widen(x[0], x[1], vs[0], vs[1]), pop, acc[t]);
+        }
+      };
+      // Step j: chunk j has landed (only the loads of later chunks, and a flush's stores,
+      // may be in flight); the stage of j - 1, whose reads have returned, takes chunk
+      // j + kStages - 1.
+      bool flushed = false;
+      int left = per - j0;  // chunks to the split's end (j0 > 0 only in the row's first)
+      auto step = [&](int j, auto now_c) __attribute__((always_inline)) {
+        constexpr int now = decltype(now_c)::value;
+        // A flush in the last step put at least DT stores behind the loads of j and j + 1.
+        const int later = min(kStages - 2, j1 - 1 - j);
+        if (flushed) {
+          if (kStages > 3 && later == 2) wait_loads<4 * NI + DT>();
+          else if (kStages > 2 && later == 1) wait_loads<2 * NI + DT>();
+          else wait_loads<DT>();
+        } else {
+          if (kStages > 3 && later == 2) wait_loads<4 * NI>();
+          else if (kStages > 2 && later == 1) wait_loads<2 * NI>();
+          else wait_loads<0>();
+        }
+        flushed = false;
+        if (j == j0) scales();
+        if (j + kStages - 1 < j1) load(j + kStages - 1, std::integral_constant<int, (now + kStages - 1) % kStages>{});
+        attend(j, now_c);
+        wait_lds();
+        if (--left == 0) {
+          flush();
+          left = per;
+          flushed = true;
+        }
+      };
+      static_assert(kStages >= 2 && kStages <= 4, "the waits above");
+      auto each_stage = [&](auto f) __attribute__((always_inline)) {
+        f(std::integral_constant<int, 0>{});
+        f(std::integral_constant<int, 1>{});
+        if constexpr (kStages > 2) f(std::integral_constant<int, 2>{});
+        if constexpr (kStages > 3) f(std::integral_constant<int, 3>{});
+      };
+      each_stage([&](auto st) __attribute__((always_inline)) {
+        if (decltype(st)::value < kStages - 1 && j0 + decltype(st)::value < j1) load(j0 + decltype(st)::value, st);
+      });
+      for (int j = j0; j < j1; j += kStages)
+        each_stage([&](auto st) __attribute__((always_inline)) {
+          if (j + decltype(st)::value < j1) step(j + decltype(st)::value, st);
+        });
+    }
+    if (split < it.split + it.splits) flush();  // the row's last split, or a long one
+  }
 }
 
-// One wave per (row, q head): the splits' partials in split order. ND dims a lane.
-template <typename T, int ND>
+// The partials of a (row, q head), ND dims a lane: up to kGroup splits by one wave, in
+// split order with all loads in flight at once; more by WAVES waves, a group each, whose
+// sums are added in order (so that the result does not depend on WAVES).
+constexpr int kGroup = 16;
+template <typename T, int ND, int WAVES>
 __global__ __launch_bounds__(256) void merge_q8_kernel(DecodeQ8Args a) {
+  constexpr int kHeads = 4 / WAVES;  // of a workgroup
   const int lane = threadIdx.x & 63;
-  const int head = blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int wave = threadIdx.x >> 6;
+  const int head = blockIdx.x * kHeads + wave / WAVES;
+  const int group = wave % WAVES;
   const int64_t row = a.d.row_base + blockIdx.y;
   if (head >= a.d.q_heads) return;
   int64_t trow, qrow;
@@ -524,30 +703,39 @@ __global__ __launch_bounds__(256) void merge_q8_kernel(DecodeQ8Args a) {
   const PartitionQ8 P = partition_q8(n, a);
   if (P.nsplit <= 1) return;
   const int64_t idx = (row * a.d.q_heads + head) * a.slots;
+  const int s0 = kGroup * group;
+  const float* src = a.d.part_acc + (idx + s0) * a.d.head_dim;
+  float x[kGroup][ND];
+#pragma unroll
+  for (int u = 0; u < kGroup; ++u)
+#pragma unroll
+    for (int j = 0; j < ND; ++j) {
+      const int d = lane + 64 * j;
+      x[u][j] = s0 + u < P.nsplit && d < a.d.head_dim ? src[u * a.d.head_dim + d] : 0.f;
+    }
   const float mi = lane < P.nsplit ? a.d.part_ml[(idx + lane) * 2] : -INFINITY;
   const float li = lane < P.nsplit ? a.d.part_ml[(idx + lane) * 2 + 1] : 0.f;
   const float M = wave_max(mi);
   const float wi = lane < P.nsplit ? fast_exp2(mi - M) : 0.f;
   const float inv = 1.f / wave_sum(wi * li);
-  const float* src = a.d.part_acc + idx * a.d.head_dim;
   float acc[ND] = {};
-  constexpr int kAhead = 8;
-  for (int s0 = 0; s0 < P.nsplit; s0 += kAhead) {
-    float x[kAhead][ND];
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u)
-#pragma unroll
-      for (int j = 0; j < ND; ++j) {
-        const int d = lane + 64 * j;
-        x[u][j] = s0 + u < P.nsplit && d < a.d.head_dim ? src[(int64_t)(s0 + u) * a.d.head_dim + d] : 0.f;
-      }
-#pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      if (s0 + u >= P.nsplit) break;
-      const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wi), s0 + u));
+  for (int u = 0; u < kGroup; ++u) {
+    const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wi), s0 + u));
+    if (s0 + u < P.nsplit) {
 #pragma unroll
       for (int j = 0; j < ND; ++j) acc[j] = fmaf(w, x[u][j], acc[j]);
     }
+  }
+  if constexpr (WAVES > 1) {
+    __shared__ float sums[WAVES][ND][64];
+#pragma unroll
+    for (int j = 0; j < ND; ++j) sums[group][j][lane] = acc[j];
+    __syncthreads();
+    if (group > 0) return;
+    for (int g = 1; g * kGroup < P.nsplit; ++g)
+#pragma unroll
+      for (int j = 0; j < ND; ++j) acc[j] += sums[g][j][lane];
   }
   T* out = reinterpret_cast<T*>(a.d.out) + qrow * a.d.o_row + (int64_t)head * a.d.o_head;
 #pragma unroll
@@ -569,11 +757,20 @@ void launch_valu(bool wide16, bool wide4, dim3 grid, hipStream_t s, const Decode
     hipLaunchKernelGGL((paged_decode_q8_kernel<T, 1, 64, 4>), grid, dim3(64), 0, s, a);
 }
 
+template <typename T, int ND>
+void launch_merge_nd(unsigned rows, hipStream_t s, const DecodeQ8Args& a) {
+  static_assert(kMaxSplitsQ8 <= 4 * kGroup, "groups of a row");
+  if (a.slots <= kGroup)
+    hipLaunchKernelGGL((merge_q8_kernel<T, ND, 1>), dim3((unsigned)ceil_div(a.d.q_heads, 4), rows), dim3(256), 0, s, a);
+  else
+    hipLaunchKernelGGL((merge_q8_kernel<T, ND, 4>), dim3((unsigned)a.d.q_heads, rows), dim3(256), 0, s, a);
+}
+
 template <typename T>
-void launch_merge_q8(dim3 grid, hipStream_t s, const DecodeQ8Args& a) {
-  if (a.d.head_dim <= 64) hipLaunchKernelGGL((merge_q8_kernel<T, 1>), grid, dim3(256), 0, s, a);
-  else if (a.d.head_dim <= 128) hipLaunchKernelGGL((merge_q8_kernel<T, 2>), grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL((merge_q8_kernel<T, 4>), grid, dim3(256), 0, s, a);
+void launch_merge_q8(unsigned rows, hipStream_t s, const DecodeQ8Args& a) {
+  if (a.d.head_dim <= 64) launch_merge_nd<T, 1>(rows, s, a);
+  else if (a.d.head_dim <= 128) launch_merge_nd<T, 2>(rows, s, a);
+  else launch_merge_nd<T, 4>(rows, s, a);
 }
 
 template <typename T>
@@ -589,10 +786,13 @@ int64_t most_pages(int32_t table_width, int32_t block_size, int32_t window) {
   const int64_t pages = window > 0 ? std::min<int64_t>(table_width, (int64_t)window / block_size + 2) : table_width;
   return std::max<int64_t>(1, pages);
 }
-int split_pages(int32_t block_size) { return std::max(1, kSplitTokens / block_size); }
+int split_pages(int32_t tokens, int32_t block_size) { return std::max(1, tokens / block_size); }
 int most_splits_q8(int32_t table_width, int32_t block_size, int32_t window) {
   const int64_t pages = most_pages(table_width, block_size, window);
-  return (int)std::min<int64_t>(kMaxSplitsQ8, ceil_div64(pages, split_pages(block_size)));
+  const int64_t short_pages = std::min<int64_t>(pages, kShortTokens / block_size);
+  int64_t most = std::max<int64_t>(1, ceil_div64(short_pages, split_pages(kSplitTokens, block_size)));
+  if (pages > short_pages) most = std::max(most, ceil_div64(pages, split_pages(kLongTokens, block_size)));
+  return (int)std::min<int64_t>(kMaxSplitsQ8, most);
 }
 
 size_t ml_bytes(int64_t slots) { return ((size_t)slots * 2 * sizeof(float) + 255) & ~(size_t)255; }
@@ -665,46 +865,57 @@ int vrh_decode_rows_q8(const Q8Call& c, const int32_t* cu_q, int32_t num_seqs, i
   a.d.block_size = c.block_size;
   a.d.bs_shift = (c.block_size & (c.block_size - 1)) == 0 ? __builtin_ctz((unsigned)c.block_size) : -1;
   a.d.window = window;
-  a.d.min_bps = split_pages(c.block_size);
+  a.d.min_bps = split_pages(kSplitTokens, c.block_size);
+  a.d.long_bps = split_pages(kLongTokens, c.block_size);
+  a.d.short_pages = kShortTokens / c.block_size;
   a.d.table_width = c.table_width;
   a.d.scale_log2 = (float)(1.4426950408889634 / std::sqrt((double)c.head_dim));
   auto cache_aligned = [&](int v) {
     return c.head_dim % v == 0 && c.c_block % v == 0 && c.c_token % v == 0 && c.c_head % v == 0 &&
            (uintptr_t)c.k % v == 0 && (uintptr_t)c.v % v == 0;
   };
-  // The matrix kernel: 16-bit queries, head_dim 64 or 128, whole 16-token steps of a
-  // page, 16-byte aligned rows, scale pairs that do not straddle a word, row offsets
+  // The matrix kernel: 16-bit queries, head_dim 64 or 128, blocks of a power of two of
+  // tokens from 16 on, 16-byte aligned rows, scale pairs that do not straddle a word, row offsets
   // within a load instruction in 32 bits.
   const bool mfma = c.dtype != VRH_DTYPE_F32 && (c.head_dim == 64 || c.head_dim == 128) &&
-                    c.block_size % 16 == 0 && c.block_size <= 65536 && cache_aligned(16) && c.c_token < (1 << 26) &&
+                    a.d.bs_shift >= 4 && c.block_size <= 65536 && cache_aligned(16) && c.c_token < (1 << 26) &&
                     c.c_token >= 0 && c.c_block >= 0 && c.q_row % 8 == 0 && c.q_head % 8 == 0 &&
                     c.o_row % 4 == 0 && c.o_head % 4 == 0 && (uintptr_t)c.q % 16 == 0 &&
                     (uintptr_t)c.out % 8 == 0 && c.s_block % 2 == 0 && c.s_head % 2 == 0 &&
                     (uintptr_t)c.scales % 2 == 0;
   a.tiles = ceil_div(a.d.group, 16);
   a.units = c.kv_heads * a.tiles;
+  auto shift_of = [](int x) { return (x & (x - 1)) == 0 ? __builtin_ctz((unsigned)x) : -1; };
+  a.min_shift = shift_of(a.d.min_bps);
+  a.long_shift = shift_of(a.d.long_bps);
+  a.split_unit = mfma ? std::max(1, kChunk / c.block_size) : 1;
+  a.compact = mfma && rows <= kCompactRows;
   const int64_t per_row = mfma ? (int64_t)a.units * a.slots : 1;
   VRH_CHECK_ARG(per_row < (1ll << 30), "%s: too many heads", who);
   const int64_t kRowsPerLaunch = std::min<int64_t>(65535, (1ll << 31) / per_row - 1);
   for (int64_t first = 0; first < rows; first += kRowsPerLaunch) {
     a.d.row_base = first;
     const unsigned count = (unsigned)std::min<int64_t>(rows - first, kRowsPerLaunch);
+    // Waves of the matrix kernel that are resident at once, by LDS.
+    constexpr int64_t kCus = 256, kLds = 160 * 1024;
+    const int64_t resident = kCus * (kLds / (kStages * 2 * kChunk * c.head_dim + 1024)) / a.units * a.units;
+    const int64_t waves = a.compact ? std::min<int64_t>(count * per_row, std::max<int64_t>(kRounds * resident, a.units))
+                                    : count * per_row;
     const dim3 grid((unsigned)a.slots, (unsigned)c.q_heads, count);
-    const dim3 mgrid((unsigned)ceil_div(c.q_heads, 4), count);
     switch (c.dtype) {
       case VRH_DTYPE_F32:
         launch_valu<float>(cache_aligned(16), cache_aligned(4), grid, s, a);
-        if (a.slots > 1) launch_merge_q8<float>(mgrid, s, a);
+        if (a.slots > 1) launch_merge_q8<float>(count, s, a);
         break;
       case VRH_DTYPE_F16:
-        if (mfma) launch_mfma_q8<f16_t>((unsigned)(count * per_row), s, a);
+        if (mfma) launch_mfma_q8<f16_t>((unsigned)waves, s, a);
         else launch_valu<f16_t>(cache_aligned(16), cache_aligned(4), grid, s, a);
-        if (a.slots > 1) launch_merge_q8<f16_t>(mgrid, s, a);
+        if (a.slots > 1) launch_merge_q8<f16_t>(count, s, a);
         break;
       default:
-        if (mfma) launch_mfma_q8<bf16_t>((unsigned)(count * per_row), s, a);
+        if (mfma) launch_mfma_q8<bf16_t>((unsigned)waves, s, a);
         else launch_valu<bf16_t>(cache_aligned(16), cache_aligned(4), grid, s, a);
-        if (a.slots > 1) launch_merge_q8<bf16_t>(mgrid, s, a);
+        if (a.slots > 1) launch_merge_q8<bf16_t>(count, s, a);
     }
   }
   VRH_RETURN_LAUNCH(who);
