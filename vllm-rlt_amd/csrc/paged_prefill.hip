@@ -569,6 +569,52 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerEu, kWavesPerEu))) void paged_prefil
       lds_dma16(vp[r], __builtin_amdgcn_readfirstlane(vl + 1024 * kWaves * r));
     }
   };
+  // The same for the 8-bit cache (block sizes are powers of two, K and V share strides).
+  // Nothing but lane_koff is kept per lane: registers spilled here would be reloaded
+  // between the staging loads, and vmcnt waits for a reload are waits for all of them.
+  auto dma8 = [&](int j, auto stage_c) __attribute__((always_inline)) {
+    constexpr int stage = decltype(stage_c)::value;
+    const uint32_t kl = lds_offset(ks[stage]) + 1024 * wave;
+    const uint32_t vl = lds_offset(vs[stage]) + 1024 * wave;
+    const int k0 = j * kSB;
+    if (((min(k0 + kSB, end) - 1) >> a.bs_shift) >= tbl_base + kTableSeg) load_table(k0 >> a.bs_shift);
+    if (kPow2 && a.uniform_pages && lane_off32 && k0 + kSB <= end) {
+      // IR whole rows of one page per instruction: a scalar address.
+      uint64_t off[NI];
+#pragma unroll
+      for (int r = 0; r < NI; ++r) {
+        const int inst = min(wave + kWaves * r, SB_INST - 1);
+        const int pb = k0 + IR * inst;
+        const uint32_t page = __builtin_amdgcn_readfirstlane(tbl_lds[(pb >> a.bs_shift) - tbl_base]);
+        const uint32_t row_off = __builtin_amdgcn_readfirstlane(pb & (a.block_size - 1));
+        off[r] = (uint64_t)page * (uint64_t)a.k_block + (uint64_t)row_off * (uint32_t)a.k_token;
+      }
+#pragma unroll
+      for (int r = 0; r < NI; ++r) {
+        if (SB_INST % kWaves != 0 && wave + kWaves * r >= SB_INST) continue;
+        lds_dma16_s(kg + off[r], lane_koff, __builtin_amdgcn_readfirstlane(kl + 1024 * kWaves * r));
+        lds_dma16_s(vg + off[r], lane_koff, __builtin_amdgcn_readfirstlane(vl + 1024 * kWaves * r));
+      }
+      return;
+    }
+    // Keys past `end` read key end - 1 again; the softmax masks them.
+#pragma unroll
+    for (int r = 0; r < NI; ++r) {
+      if (SB_INST % kWaves != 0 && wave + kWaves * r >= SB_INST) continue;
+      const int v = 64 * (wave + kWaves * r) + lane;
+      const int row = v / KCH;
+      const int pos = min(k0 + row, end - 1);
+      const int64_t off = (int64_t)tbl_lds[(pos >> a.bs_shift) - tbl_base] * a.k_block +
+                          (int64_t)(pos & (a.block_size - 1)) * a.k_token +
+                          (((v % KCH) ^ L::swizzle(row)) * CPE);
+      lds_dma16(kg + off, __builtin_amdgcn_readfirstlane(kl + 1024 * kWaves * r));
+      lds_dma16(vg + off, __builtin_amdgcn_readfirstlane(vl + 1024 * kWaves * r));
+    }
+  };
+  auto stage_keys = [&](int j, auto stage_c) __attribute__((always_inline)) {
+    if constexpr (kQ8) dma8(j, stage_c);
+    else dma(j, stage_c);
+  };
   // Per-lane LDS byte offsets inside a half-stage (the swizzle depends on
   // row & 15, which the 16-key steps below leave unchanged):
   //  * K operand reads: row `col`, dims 16c + 8half;
@@ -777,8 +823,8 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerEu, kWavesPerEu))) void paged_prefil
       return;
     }
     // A value that a query does not see must not reach it, and 0 * NaN would: where the
-    // mask is at work, NaN values are taken out of the product, and (rarely) a product of
-    // their places with the mask finds the queries that do see them.
+    // mask is at work, NaN values are taken out of the product, and given (rarely) to the
+    // queries that do see them.
     uint32_t found = 0;
 #pragma unroll
     for (int i = 0; i < 2 * DB; ++i) {
@@ -788,43 +834,32 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerEu, kWavesPerEu))) void paged_prefil
       acc[i % DB] = Mfma<T>::run(MfmaQ8<T>::widen(x[0] & ~(b0 * 0xFF), x[1] & ~(b1 * 0xFF), vscale[i / DB],
                                                   vscale[i / DB]),
                                  pop[i / DB], acc[i % DB]);
+      __builtin_amdgcn_sched_barrier(0);  // one operand at a time: registers
     }
     if (!__any(found != 0)) return;
-    const int bound = (q_ok ? min(qpos, end - 1) : -1) - j * kSB - 4 * half;
-    u32x4 seen[2];
-#pragma unroll
-    for (int c = 0; c < 2; ++c)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int key = 16 * c + 8 * (i >> 1) + 2 * (i & 1);
-        seen[c][i] = pack2<bf16_t>(key <= bound ? 1.f : 0.f, key + 1 <= bound ? 1.f : 0.f);
-      }
+    // Lane dims 32 db + 8 gi + 4 half .. + 3, key by key: slow, but it holds no registers
+    // that the loop around it would have to spill.
+    const int seen = (q_ok ? min(qpos, end - 1) : -1) - j * kSB;
 #pragma unroll 1
-    for (int db = 0; db < DB; ++db) {
-      f32x16 hit = {};
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const u32x2 x = lds_read_tr8(vd + 16 * c * D + Lds8<D>::chunk(vb8, db));
-        hit = Mfma<bf16_t>::run(
-            MfmaQ8<bf16_t>::widen(nan_bytes(x[0]) * 0x38, nan_bytes(x[1]) * 0x38, 1.f, 1.f), seen[c], hit);
-      }
-      uint32_t bits = 0;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) bits |= (hit[e] > 0.f ? 1u : 0u) << e;
-      poison_lds[db][tid] |= (uint16_t)bits;
+    for (int i = 0; i < 4 * DB * kSB; ++i) {
+      const int key = i / (4 * DB), db = i / 4 % DB, gi = i % 4;
+      const uint32_t at = key * D + 16 * ((2 * db + (gi >> 1)) ^ Lds8<D>::swizzle(key)) + 8 * (gi & 1) + 4 * half;
+      const uint32_t bad = nan_bytes(*reinterpret_cast<const uint32_t*>(vd + at));
+      const uint32_t bits = (bad & 1) | (bad >> 7 & 2) | (bad >> 14 & 4) | (bad >> 21 & 8);
+      if (bits != 0 && key <= seen) poison_lds[db][tid] |= (uint16_t)(bits << (4 * gi));
     }
     poisoned = true;
   };
   if (j0 < nsub) {
-    dma(j0, H0{});
-    if (j0 + 1 < nsub) dma(j0 + 1, H1{});
+    stage_keys(j0, H0{});
+    if (j0 + 1 < nsub) stage_keys(j0 + 1, H1{});
     auto step = [&](int j, auto hc) {
       constexpr int h = decltype(hc)::value;
       using Hd = std::integral_constant<int, (h + 2) % kStages>;
       if (j + 1 < nsub) dma_wait_newest();
       else vm_wait<0>();
       __syncthreads();
-      if (j + 2 < nsub) dma(j + 2, Hd{});
+      if (j + 2 < nsub) stage_keys(j + 2, Hd{});
       if (j >= nsub_w) return;
       const char* kd = reinterpret_cast<const char*>(ks[h]);
       f32x16 st = f32x16{};
@@ -1069,7 +1104,8 @@ bool launch_prefill_d(int d, dim3 grid, hipStream_t s, const PrefillArgs& a) {
 template <typename T, typename C = T>
 bool launch_prefill(int d, dim3 grid, hipStream_t s, const PrefillArgs& a) {
   if (a.bs_shift >= 0) return launch_prefill_d<T, C, kShift>(d, grid, s, a);
-  return launch_prefill_d<T, C, kDiv>(d, grid, s, a);
+  if constexpr (std::is_same<T, C>::value) return launch_prefill_d<T, C, kDiv>(d, grid, s, a);
+  return false;  // the 8-bit cache's tiles are asked for powers of two only
 }
 
 }  // namespace
@@ -1392,9 +1428,9 @@ size_t rows_bytes_q8(int64_t num_seqs, int32_t max_seqlen_q, int32_t q_heads, in
           255) / 256 * 256;
 }
 bool tiles_q8(int dtype, int32_t head_dim, int32_t block_size) {
-  // Scales are looked up once per 16 keys.
+  // Scales are looked up once per 16 keys, pages by shifts.
   return (dtype == VRH_DTYPE_BF16 || dtype == VRH_DTYPE_F16) && tile_head_dim(head_dim) &&
-         block_size >= 16 && block_size % 16 == 0 && block_size <= 65536;
+         block_size >= 16 && (block_size & (block_size - 1)) == 0 && block_size <= 65536;
 }
 }  // namespace
 
