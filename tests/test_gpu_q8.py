@@ -306,6 +306,51 @@ def test_decode_rows_do_not_depend_on_the_batch(gpu, dtype, hq, hkv, dim):
         assert torch.equal(alone[0], batch[r])
 
 
+@pytest.mark.parametrize("rows,most,hq,hkv,dtype,dim", [
+    (65, 900, 4, 4, torch.bfloat16, 64),  # more rows than a wave counts at once
+    (200, 2600, 16, 16, torch.bfloat16, 128),  # more splits than waves: shares of several
+    (512, 300, 16, 2, torch.float16, 64),
+    (513, 300, 4, 1, torch.bfloat16, 128),  # beyond the rows that are counted
+    (700, 200, 2, 2, torch.float32, 64),
+])
+def test_decode_of_many_rows(gpu, rows, most, hq, hkv, dtype, dim):
+    from vllm_rlt.kernels.hip_attention_q8 import paged_attention_q8
+
+    rng = np.random.default_rng(rows)
+    lengths = [int(n) for n in rng.integers(0, most, rows)]
+    lengths[0], lengths[rows // 2], lengths[-1] = most, 0, most - 1
+    # Rows share pages: the pool needs no more than the longest.
+    tables, blocks = tables_of(rng, [most] * 4, 16)
+    tables = tables[rng.integers(0, 4, rows)]
+    layer = Layer(gpu, blocks, 16, hkv, dim)
+    q = torch.randn((rows, hq, dim), generator=torch.Generator().manual_seed(4)).to(dtype).to(gpu)
+    got = paged_attention_q8(q, *layer.args, ints(tables, gpu), ints(lengths, gpu))
+    for r in {0, 1, 63, 64, rows // 2, rows // 2 + 1, rows - 2, rows - 1}:
+        alone = paged_attention_q8(q[r : r + 1], *layer.args, ints(tables[r : r + 1], gpu),
+                                   ints(lengths[r : r + 1], gpu))
+        assert torch.equal(alone[0], got[r]), r
+    assert got.isfinite().all() and not got[rows // 2].any()
+    for r in (0, rows - 1):
+        want = ref.attend(to64(q[r : r + 1]), *layer.context(tables[r], lengths[r]), lengths[r] - 1)
+        check_attention(got[r : r + 1], *want, dtype, dim, lengths[r])
+
+
+@pytest.mark.parametrize("dtype,bs,n", [(torch.bfloat16, 16, 70001), (torch.float16, 32, 140000),
+                                        (torch.float32, 16, 70001), (torch.bfloat16, 128, 9000)])
+def test_decode_of_one_very_long_row(gpu, dtype, bs, n):
+    """Splits of more pages than a wave keeps ids of."""
+    from vllm_rlt.kernels.hip_attention_q8 import paged_attention_q8
+
+    rng = np.random.default_rng(3)
+    tables, blocks = tables_of(rng, [n], bs)
+    layer = Layer(gpu, blocks, bs, 1, 64)
+    q = torch.randn((1, 3, 64), generator=torch.Generator().manual_seed(4)).to(dtype)
+    for window in (0, n - 5):
+        got = paged_attention_q8(q.to(gpu), *layer.args, ints(tables, gpu), ints([n], gpu), window)
+        want = ref.attend(to64(q), *layer.context(tables[0], n), n - 1, window)
+        check_attention(got, *want, dtype, 64, n)
+
+
 def test_decode_in_a_pool_past_32_bit_offsets(gpu):
     """Blocks more than 2^31 and 2^32 bytes into the cache."""
     from vllm_rlt.kernels.hip_attention_q8 import kv_append_q8, kv_read_q8, paged_attention_q8

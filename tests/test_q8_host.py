@@ -35,13 +35,15 @@ def test_every_touched_page_has_a_slot_of_its_sequence():
             for slot in range(int(cu[-1]) // bs + 2 * len(counts)):
                 # The search of 64 candidates at a time.
                 lo, hi, found = 0, len(counts), True
-                while hi - lo > 1:
+                while True:
                     step = (hi - lo + 63) // 64
                     at = [lo + i * step < hi and base[lo + i * step] <= slot for i in range(64)]
                     if not any(at):
                         found = False
                         break
                     lo += max(i for i in range(64) if at[i]) * step
+                    if step == 1:
+                        break
                     hi = min(hi, lo + step)
                 want = [s for s in range(len(counts)) if base[s] <= slot]
                 if found and slot >= base[lo]:
@@ -131,5 +133,5 @@ def test_workspaces_follow_the_shapes():
     assert size(4, 16, 128, 16, 8, 0) == 0  # one split of 128 tokens: written by its wave
     assert size(0, 16, 128, 16, 800, 0) == 0
     assert 0 < size(4, 16, 128, 16, 800, 512) < size(4, 16, 128, 16, 800, 0)
-    assert size(4, 16, 128, 16, 800, 0) == size(4, 16, 128, 16, 8000, 0)  # splits are bounded
+    assert size(4, 16, 128, 16, 2000, 0) == size(4, 16, 128, 16, 8000, 0)  # splits are bounded
     assert size(8, 16, 128, 16, 800, 0) == 2 * size(4, 16, 128, 16, 800, 0)

@@ -38,27 +38,51 @@ struct Q8AppendArgs {
 
 // A wave's page: the first page slots of sequence s are floor(cu[s] / bs) + 2 s, which
 // leaves it at least as many as its q tokens can touch (floor(q / bs) + 2), so that a
-// slot finds its sequence without a prefix sum of pages. 64 candidates at a time.
-__device__ __forceinline__ bool q8_slot(const Q8AppendArgs& a, int64_t slot, int64_t& seq, int& page_idx) {
+// slot finds its sequence without a prefix sum of pages. 64 candidates at a time; what
+// is needed of the last 64 sequences is loaded with them, so that up to 64 sequences
+// cost one round trip to memory.
+struct Q8Slot {
+  int64_t seq, row0, q, n;  // the sequence, its first row, rows and length
+  int page_idx;
+};
+__device__ __forceinline__ int64_t pick64(int64_t x, int lane) {
+  return ((int64_t)__builtin_amdgcn_readlane((int)(x >> 32), lane) << 32) |
+         (uint32_t)__builtin_amdgcn_readlane((int)x, lane);
+}
+__device__ __forceinline__ bool q8_slot(const Q8AppendArgs& a, int64_t slot, Q8Slot& s) {
   const int lane = threadIdx.x & 63;
   if (a.cu == nullptr) {
-    seq = slot;
-    page_idx = 0;
-    return slot < a.num_seqs;
+    if (slot >= a.num_seqs) return false;
+    s = {slot, slot, 1, a.lengths[slot], 0};
+    return true;
   }
   int64_t lo = 0, hi = a.num_seqs;  // the sequence is in [lo, hi)
-  while (hi - lo > 1) {
+  for (;;) {
     const int64_t step = (hi - lo + 63) / 64;
     const int64_t mine = lo + lane * step;
-    const bool at = mine < hi && a.cu[mine] / a.block_size + 2 * mine <= slot;
-    const uint64_t hit = __ballot(at);
+    int64_t first = 0;
+    int q = 0, n = 0;
+    if (mine < hi) {
+      first = a.cu[mine];
+      if (step == 1) {
+        q = a.cu[mine + 1] - (int)first;
+        n = a.lengths[mine];
+      }
+    }
+    const uint64_t hit = __ballot(mine < hi && first / a.block_size + 2 * mine <= slot);
     if (hit == 0) return false;
-    lo += (63 - __builtin_clzll(hit)) * step;
+    const int pick = 63 - __builtin_clzll(hit);
+    lo += pick * step;
+    if (step == 1) {
+      s.seq = lo;
+      s.row0 = pick64(first, pick);
+      s.q = __builtin_amdgcn_readlane(q, pick);
+      s.n = __builtin_amdgcn_readlane(n, pick);
+      s.page_idx = (int)(slot - (s.row0 / a.block_size + 2 * lo));
+      return true;
+    }
     hi = min(hi, lo + step);
   }
-  seq = lo;
-  page_idx = (int)(slot - (a.cu[lo] / a.block_size + 2 * lo));
-  return page_idx >= 0;
 }
 
 template <typename T, int VE>
@@ -111,22 +135,19 @@ __global__ __launch_bounds__(256) void kv_append_q8_kernel(Q8AppendArgs a) {
   const int item = (int)__builtin_amdgcn_readfirstlane(blockIdx.y * 4 + (threadIdx.x >> 6));
   if (item >= 2 * a.heads) return;
   const int head = item >> 1, part = item & 1;
-  int64_t seq;
-  int page_idx;
-  if (!q8_slot(a, blockIdx.x, seq, page_idx)) return;
-  const int64_t row0 = a.cu ? a.cu[seq] : seq;
-  const int64_t q = a.cu ? a.cu[seq + 1] - row0 : 1;
-  const int64_t n = a.lengths[seq];
+  Q8Slot at;
+  if (!q8_slot(a, blockIdx.x, at)) return;
+  const int64_t row0 = at.row0, q = at.q, n = at.n;
   if (q <= 0 || n <= 0) return;
   // Positions before 0 or past the table take no row.
   const int64_t before = n - q;  // may be negative: then the first rows have no position
   const int64_t first = before > 0 ? before : 0;
   const int64_t cap = (int64_t)a.table_width * a.block_size;
   const int64_t end = n < cap ? n : cap;
-  const int64_t page = first / a.block_size + page_idx;
+  const int64_t page = first / a.block_size + at.page_idx;
   const int64_t p0 = page * a.block_size;
   if (p0 >= end) return;
-  const int64_t block = a.tables[seq * a.table_stride + page];
+  const int64_t block = a.tables[at.seq * a.table_stride + page];
   if (block < 0 || block >= a.num_blocks) return;
   const int old = (int)max((int64_t)0, first - p0);  // older tokens of the page
   const int stop = (int)min((int64_t)a.block_size, end - p0);

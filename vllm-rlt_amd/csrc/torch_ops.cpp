@@ -522,6 +522,8 @@ Metadata sequence_metadata(const at::Tensor& tables, const at::Tensor& rows_in,
   const c10::DeviceGuard guard(tables.device());
   const at::Tensor rows = rows_in.contiguous(), lengths = lengths_in.contiguous(),
                    counts = counts_in.contiguous();
+  // Outputs of the op itself: nothing here is for autograd to see.
+  const at::AutoDispatchBelowADInplaceOrView below;
   const auto ints = tables.options();
   const at::Tensor wide = at::empty({3, tokens}, ints.dtype(at::kLong));
   at::Tensor mask = at::empty({tokens}, ints.dtype(at::kBool));
@@ -537,7 +539,7 @@ Metadata sequence_metadata(const at::Tensor& tables, const at::Tensor& rows_in,
                                  (int32_t)tables.size(1), (int32_t)out_width, (int32_t)page,
                                  stream_of(tables)),
            "vrh_sequence_metadata");
-  return {wide[0], wide[1], wide[2], mask, out_tables, narrow.narrow(0, 0, n), narrow.narrow(0, n, n + 1)};
+  return {wide.select(0, 0), wide.select(0, 1), wide.select(0, 2), mask, out_tables, narrow.narrow(0, 0, n), narrow.narrow(0, n, n + 1)};
 }
 
 }  // namespace
