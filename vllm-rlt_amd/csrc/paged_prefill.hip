@@ -67,6 +67,7 @@ typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef __attribute__((ext_vector_type(4))) float f32x4;
 typedef __attribute__((ext_vector_type(4))) uint32_t u32x4;
 typedef __attribute__((ext_vector_type(2))) uint32_t u32x2;
+typedef __attribute__((ext_vector_type(8))) int i32x8;
 
 // 32x32x16 MFMA: A lane l = row l % 32 with k-slots 8 * (l / 32) + i, B lane
 // l = column l % 32 with the same k-slots; D lane l = column l % 32, element j
@@ -281,6 +282,8 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerEu, kWavesPerEu))) void paged_prefil
   constexpr int DC = D / 16;                   // 16-wide d chunks (QK^T k-steps)
   constexpr int DB = D / 32;                   // 32-row d blocks of O^T
   constexpr bool kQ8 = sizeof(C) == 1;
+  // K bytes go into e4m3 MFMAs as they are, against Q in two e4m3 pieces.
+  constexpr bool kQk8 = kQ8 && std::is_same<T, bf16_t>::value && D % 64 == 0;
   constexpr int KCH = D * (int)sizeof(C) / 16; // 16-byte chunks per key row
   constexpr int CPE = 16 / (int)sizeof(C);     // elements per chunk
   constexpr int SB_INST = kSB * KCH / 64;      // 16-byte wave stores per sub-block (K or V)
@@ -380,7 +383,7 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerEu, kWavesPerEu))) void paged_prefil
   // Q^T B-operands: lane holds query `col`, dims 16c + 8*half .. +8 (8-bit cache: k-steps
   // 2c and 2c + 1 are the halves of one 16-byte K read, dims 32c + 16*half .. +16).
   u32x4 qop[DC];
-  {
+  if constexpr (!kQk8) {
     const T* qp = reinterpret_cast<const T*>(a.q) + (int64_t)(q_begin + (q_ok ? qi : 0)) * a.q_token +
                   head * a.q_head + (kQ8 ? 16 : 8) * half;
 #pragma unroll
@@ -389,6 +392,48 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerEu, kWavesPerEu))) void paged_prefil
           *reinterpret_cast<const u32x4*>(qp + (kQ8 ? 32 * (c >> 1) + 8 * (c & 1) : 16 * c));
       qop[c] = q_ok ? v : u32x4{0, 0, 0, 0};
     }
+  }
+
+  // Q in e4m3 pieces q1 + q2 2^-4, times 2^(q_exp - 127): bf16 has 8 significant bits, a
+  // piece 4 (and q2 a sign of its own), so this is Q itself down to 2^-22 of the row's
+  // largest value, at the cost in MFMA cycles of one bf16 product and without widening
+  // K: the 32 conversions of a sub-block were a ninth of the kernel's time. f16 has 11
+  // bits, a third piece more than the conversions cost.
+  i32x8 q8op[kQk8 ? D / 64 : 1][2];
+  int q_exp = 0;
+  if constexpr (kQk8) {
+    // Lane: query `col`, dims 64c + 32 half .. + 31 of k-step c.
+    const T* qp = reinterpret_cast<const T*>(a.q) + (int64_t)(q_begin + (q_ok ? qi : 0)) * a.q_token +
+                  head * a.q_head + 32 * half;
+    float top = 0.f;
+    u32x4 raw[D / 64][4];
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const u32x4 v = *reinterpret_cast<const u32x4*>(qp + 64 * c + 8 * i);
+        raw[c][i] = q_ok ? v : u32x4{0, 0, 0, 0};
+        float x[8];
+        unpack<T, 8>(raw[c][i], x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(x[e]));
+      }
+    top = fmaxf(top, shfl_xor_f32(top, 32));
+    q_exp = q8_exponent(top);
+    const float inv = q8_scale(254 - min(q_exp, 254));
+#pragma unroll
+    for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+      for (int w = 0; w < 8; ++w) {  // 4 dims each
+        float x[8], y[4];
+        unpack<T, 8>(raw[c][w >> 1], x);
+        const int o = 4 * (w & 1);
+        const uint32_t hi = q8_pack4(x[o] * inv, x[o + 1] * inv, x[o + 2] * inv, x[o + 3] * inv);
+        q8_unpack4(hi, y);
+        q8op[c][0][w] = (int)hi;
+        q8op[c][1][w] = (int)q8_pack4((x[o] * inv - y[0]) * 16.f, (x[o + 1] * inv - y[1]) * 16.f,
+                                      (x[o + 2] * inv - y[2]) * 16.f, (x[o + 3] * inv - y[3]) * 16.f);
+      }
   }
 
   f32x16 acc[DB];
@@ -656,8 +701,11 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerEu, kWavesPerEu))) void paged_prefil
   const int tr8_row = ((lane >> 1) & 3) + 4 * half + 8 * ((lane >> 3) & 1);
   const uint32_t vb8 = tr8_row * D + 16 * (((lane >> 4) & 1) ^ Lds8<D>::swizzle(tr8_row)) + 8 * (lane & 1);
   // Scales of a sub-block's two 16-key halves: K's with the softmax scale, V's (v_scale).
+  // With kQk8 the score MFMAs apply K's scale: k_exp is that of key `col`.
   float kl[2], vscale[2], pscale[2];
+  int k_exp = 0;
   auto scales_of = [&](int j) {
+    if constexpr (kQk8) k_exp = scale_lds[page_of(min(j * kSB + col, end - 1)) - tbl_base] & 255;
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       const int page = page_of(min(j * kSB + 16 * t, end - 1));
@@ -672,10 +720,11 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerEu, kWavesPerEu))) void paged_prefil
   // P^T B-operands of scores `st` (already masked, m current): per 16-key
   // chunk c, elements 8c .. 8c+7 of st, i.e. keys 16c + 4half + {0..3} and
   // 16c + 8 + 4half + {0..3}.
+  constexpr bool kScaled = kQ8 && !kQk8;  // scores still lack K's scale
   auto probs = [&](const f32x16& st, u32x4 (&pop)[2]) {
     float p[16];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) p[i] = fast_exp2(fmaf(st[i], kQ8 ? kl[i >> 3] : a.scale_log2, -m));
+    for (int i = 0; i < 16; ++i) p[i] = fast_exp2(fmaf(st[i], kScaled ? kl[i >> 3] : a.scale_log2, -m));
     float w[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) w[i] = p[i];
@@ -712,7 +761,7 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerEu, kWavesPerEu))) void paged_prefil
   auto row_max = [&](int j, f32x16& st, auto masked_c) {
     const int k0 = j * kSB;
     float mx = -INFINITY;
-    if constexpr (kQ8) {
+    if constexpr (kScaled) {
       if constexpr (decltype(masked_c)::value) {
         const int bound = (q_ok ? min(qpos, end - 1) : -1) - k0 - 4 * half;
 #pragma unroll
@@ -747,7 +796,7 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerEu, kWavesPerEu))) void paged_prefil
                                                        false, false);
       mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
     }
-    const float mcand = kQ8 ? mx : mx * a.scale_log2;
+    const float mcand = kScaled ? mx : mx * a.scale_log2;
     if (__any(mcand > m + (kQ8 ? Weights<T>::kSlack : 8.f))) {
       const float mnew = fmaxf(m, kQ8 ? mcand - Weights<T>::kLift : mcand);
       const float corr = fast_exp2(m - mnew);
@@ -798,14 +847,37 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerEu, kWavesPerEu))) void paged_prefil
   auto attend8 = [&](int j, const char* kd, const char* vd) __attribute__((always_inline)) {
     scales_of(j);
     f32x16 st = f32x16{};
-    auto kread = [&](int c) { return *reinterpret_cast<const u32x4*>(kd + Lds8<D>::chunk(kb8, c)); };
-    u32x4 kop[DC / 2];
-    kop[0] = kread(0);
+    if constexpr (kQk8) {
+      // Lane: key `col`, chunks 4c + 2 half and + 1 (the k-slots of q8op).
+      const char* kp = kd + col * D;
+      const uint32_t x0 = 16 * ((2 * half) ^ Lds8<D>::swizzle(col));
+      i32x8 kop[D / 64];
 #pragma unroll
-    for (int c = 0; c < DC / 2; ++c) {
-      if (c + 1 < DC / 2) kop[c + 1] = kread(c + 1);
-      st = Mfma<T>::run(MfmaQ8<T>::widen(kop[c][0], kop[c][1], 1.f, 1.f), qop[2 * c], st);
-      st = Mfma<T>::run(MfmaQ8<T>::widen(kop[c][2], kop[c][3], 1.f, 1.f), qop[2 * c + 1], st);
+      for (int c = 0; c < D / 64; ++c) {
+        const u32x4 lo = *reinterpret_cast<const u32x4*>(kp + (x0 ^ (64 * c)));
+        const u32x4 hi = *reinterpret_cast<const u32x4*>(kp + (x0 ^ (64 * c + 16)));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          kop[c][i] = (int)lo[i];
+          kop[c][4 + i] = (int)hi[i];
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          st = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kop[c], q8op[c][i], st, 0, 0, 0, k_exp, 0,
+                                                               q_exp - 4 * i);
+    } else {
+      auto kread = [&](int c) { return *reinterpret_cast<const u32x4*>(kd + Lds8<D>::chunk(kb8, c)); };
+      u32x4 kop[DC / 2];
+      kop[0] = kread(0);
+#pragma unroll
+      for (int c = 0; c < DC / 2; ++c) {
+        if (c + 1 < DC / 2) kop[c + 1] = kread(c + 1);
+        st = Mfma<T>::run(MfmaQ8<T>::widen(kop[c][0], kop[c][1], 1.f, 1.f), qop[2 * c], st);
+        st = Mfma<T>::run(MfmaQ8<T>::widen(kop[c][2], kop[c][3], 1.f, 1.f), qop[2 * c + 1], st);
+      }
     }
     mask_max(j, st);
     u32x4 pop[2];
