@@ -78,107 +78,87 @@ __device__ __forceinline__ int wave_scan(int x) {
   return x;
 }
 
-// Work of the matrix kernel's waves. For up to kCompactRows rows the splits that exist
-// are numbered (rows in order), and a KV head's waves take equal shares of consecutive
-// ones: one split each while there are no more than kRounds times as many as waves are
-// resident, else runs of a row's splits (within kSegment pages). Which wave takes a split
-// changes no result, since each split has its own state. So no wave without work holds
-// the LDS that another waits for, however wide the tables are (48 decode rows of a mixed
-// step under tables of 512 pages: 119 us with a wave for each slot, 85). One share per
-// resident wave, no starts but the first, was slower (64 rows 117 us against 107): the
-// heads of a block, neighbours in memory, drift apart. Each wave counts the rows' splits
-// itself, 64 rows at a time; beyond kCompactRows a wave takes one split, workgroups being
-// dealt slots x rows.
-constexpr int kRounds = 8;
+// Work of the waves. For up to kCompactRows rows the splits that exist are numbered (rows
+// in order), each wave counting them itself, 64 rows at a time, and as many waves as are
+// resident take every waves-th one: none is launched without work however wide the
+// tables are (38 float32 rows of 2-21 tokens, 64 heads, under tables of 2063 pages: 137 us
+// with a wave for each slot), and the waves of a split's heads, whose pages are
+// neighbours in memory, run at the same time. Which wave takes a split changes no
+// result. Equal shares of consecutive splits, with no restart between them, were slower
+// (64 rows of 512-4096 tokens, 16 x 128 heads: 117 us against 107): the heads drift apart.
+// Beyond that many rows a wave takes one split, workgroups being dealt slots x rows.
 constexpr int kCompactRows = 512;
 constexpr int kSegment = 64;
+
+// A lane's row of up to 64 consecutive ones, and its splits.
+struct RowQ8 {
+  int64_t trow, qrow;
+  int n, splits;
+};
+__device__ __forceinline__ RowQ8 q8_row(const DecodeQ8Args& a, int64_t row) {
+  RowQ8 r = {0, 0, -1, 0};
+  if (row < a.d.rows) r.n = row_length(row, a.d, &r.trow, &r.qrow);
+  if (r.n > 0) r.splits = partition_q8(r.n, a).nsplit;
+  else if (r.n == 0) r.splits = 1;
+  return r;
+}
 
 struct ItemQ8 {
   int64_t row;   // work row
   int64_t trow;  // table row
   int64_t qrow;  // query and output row
   int n;         // visible length
-  int split, splits;  // first split, and how many
+  int split;
 };
 
-// A lane's row of up to 64 consecutive ones: its splits, and the most of them in a run.
-struct RowQ8 {
-  int64_t trow, qrow;
-  int n, splits, most;
-};
-__device__ __forceinline__ RowQ8 q8_row(const DecodeQ8Args& a, int64_t row) {
-  RowQ8 r = {0, 0, -1, 0, 1};
-  if (row < a.d.rows) r.n = row_length(row, a.d, &r.trow, &r.qrow);
-  if (r.n > 0) {
-    const PartitionQ8 P = partition_q8(r.n, a);
-    r.splits = P.nsplit;
-    r.most = (P.bps & (P.bps - 1)) == 0 ? kSegment >> (31 - __builtin_clz(P.bps)) : kSegment / P.bps;
-    r.most = max(1, r.most);
-  } else if (r.n == 0) {
-    r.splits = 1;
-  }
-  return r;
-}
-
-// A wave's share of a KV head's splits, all of it wave-uniform but `r` and `upto`.
-struct ShareQ8 {
+// A wave's walk over the splits, all of it wave-uniform but `r` and `upto`.
+struct WalkQ8 {
   RowQ8 r;          // this lane's row of the 64 from `base` on
   int upto;         // splits of those rows up to this lane's
   int64_t base;
   uint32_t before;  // splits of the rows before `base`
-  uint32_t next, end;
+  uint32_t next;
 };
 
-__device__ __forceinline__ void q8_share(const DecodeQ8Args& a, uint32_t wave, uint32_t waves, ShareQ8& s) {
-  const int lane = threadIdx.x & 63;
-  if (a.compact == 0) {
-    s.next = wave;
-    s.end = wave + 1;
-    return;
-  }
-  s.base = 0;
-  s.before = 0;
-  s.r = q8_row(a, lane);
-  s.upto = wave_scan(s.r.splits);
-  uint32_t total = (uint32_t)__builtin_amdgcn_readlane(s.upto, 63);
-  for (int64_t base = 64; base < a.d.rows; base += 64)
-    total += (uint32_t)wave_sum_i(q8_row(a, base + lane).splits);
-  s.next = (uint32_t)((uint64_t)wave * total / waves);
-  s.end = (uint32_t)((uint64_t)(wave + 1) * total / waves);
+__device__ __forceinline__ void q8_start(const DecodeQ8Args& a, uint32_t wave, WalkQ8& w) {
+  w.next = wave;
+  if (a.compact == 0) return;
+  w.base = 0;
+  w.before = 0;
+  w.r = q8_row(a, threadIdx.x & 63);
+  w.upto = wave_scan(w.r.splits);
 }
 
-// The share's next run; false when it is done.
-__device__ __forceinline__ bool q8_next(const DecodeQ8Args& a, ShareQ8& s, ItemQ8& it) {
-  if (s.next >= s.end) return false;
+// The walk's next split; false when there is none. `step`: waves that walk together.
+__device__ __forceinline__ bool q8_next(const DecodeQ8Args& a, uint32_t step, WalkQ8& w, ItemQ8& it) {
   if (a.compact == 0) {
-    it.row = a.d.row_base + s.next / (uint32_t)a.slots;
-    it.split = (int)(s.next % (uint32_t)a.slots);
-    it.splits = 1;
+    if (w.next == UINT32_MAX) return false;
+    it.row = a.d.row_base + w.next / (uint32_t)a.slots;
+    it.split = (int)(w.next % (uint32_t)a.slots);
     it.n = row_length(it.row, a.d, &it.trow, &it.qrow);
-    ++s.next;
+    w.next = UINT32_MAX;
     return true;
   }
   for (;;) {
-    const uint32_t all = (uint32_t)__builtin_amdgcn_readlane(s.upto, 63);
-    if (s.next - s.before < all) break;
-    s.before += all;
-    s.base += 64;
-    s.r = q8_row(a, s.base + (threadIdx.x & 63));
-    s.upto = wave_scan(s.r.splits);
+    const uint32_t all = (uint32_t)__builtin_amdgcn_readlane(w.upto, 63);
+    if (w.next - w.before < all) break;
+    w.before += all;
+    w.base += 64;
+    if (w.base >= a.d.rows) return false;
+    w.r = q8_row(a, w.base + (threadIdx.x & 63));
+    w.upto = wave_scan(w.r.splits);
   }
   // First lane whose splits end past the next one.
-  const uint32_t at = s.next - s.before;
-  const int pick = __builtin_ffsll((long long)__ballot((uint32_t)s.upto > at)) - 1;
-  it.row = s.base + pick;
-  it.trow = ((int64_t)__builtin_amdgcn_readlane((int)(s.r.trow >> 32), pick) << 32) |
-            (uint32_t)__builtin_amdgcn_readlane((int)s.r.trow, pick);
-  it.qrow = ((int64_t)__builtin_amdgcn_readlane((int)(s.r.qrow >> 32), pick) << 32) |
-            (uint32_t)__builtin_amdgcn_readlane((int)s.r.qrow, pick);
-  it.n = __builtin_amdgcn_readlane(s.r.n, pick);
-  const int splits = __builtin_amdgcn_readlane(s.r.splits, pick);
-  it.split = (int)at - (__builtin_amdgcn_readlane(s.upto, pick) - splits);
-  it.splits = min(min(__builtin_amdgcn_readlane(s.r.most, pick), splits - it.split), (int)(s.end - s.next));
-  s.next += (uint32_t)it.splits;
+  const uint32_t at = w.next - w.before;
+  const int pick = __builtin_ffsll((long long)__ballot((uint32_t)w.upto > at)) - 1;
+  it.row = w.base + pick;
+  it.trow = ((int64_t)__builtin_amdgcn_readlane((int)(w.r.trow >> 32), pick) << 32) |
+            (uint32_t)__builtin_amdgcn_readlane((int)w.r.trow, pick);
+  it.qrow = ((int64_t)__builtin_amdgcn_readlane((int)(w.r.qrow >> 32), pick) << 32) |
+            (uint32_t)__builtin_amdgcn_readlane((int)w.r.qrow, pick);
+  it.n = __builtin_amdgcn_readlane(w.r.n, pick);
+  it.split = (int)at - (__builtin_amdgcn_readlane(w.upto, pick) - __builtin_amdgcn_readlane(w.r.splits, pick));
+  w.next += step;
   return true;
 }
 
@@ -190,164 +170,166 @@ __device__ __forceinline__ bool q8_next(const DecodeQ8Args& a, ShareQ8& s, ItemQ
 // arithmetic is fp32: float32 queries, and every shape the matrix kernel does not take.
 template <typename T, int VE, int LPT, int ND>
 __global__ __launch_bounds__(64) void paged_decode_q8_kernel(DecodeQ8Args a) {
-  constexpr int U = VE >= 4 ? 4 : 2;
+  constexpr int U = VE >= 16 ? 8 : VE >= 4 ? 4 : 2;
   constexpr int TPL = 64 / LPT;
   constexpr int CH = U * TPL;
   using raw_t = raw_of<VE>;
   const int lane = threadIdx.x;
   const int dg = lane % LPT, tg = lane / LPT;
-  const int head = blockIdx.y;
+  const uint32_t first = blockIdx.x / (uint32_t)a.units, step = gridDim.x / (uint32_t)a.units;
+  const int head = (int)(blockIdx.x - first * (uint32_t)a.units);
   const int kvh = head / a.d.group;
-  const int64_t row = a.d.row_base + blockIdx.z;
-  int64_t trow, qrow;
-  const int n = row_length(row, a.d, &trow, &qrow);
-  if (n < 0) return;
-  T* out = reinterpret_cast<T*>(a.d.out) + qrow * a.d.o_row + (int64_t)head * a.d.o_head;
-  if (n == 0) {
-    if (blockIdx.x == 0)
-      for (int d = lane; d < a.d.head_dim; d += 64) out[d] = from_f32<T>(0.f);
-    return;
-  }
-  const PartitionQ8 P = partition_q8(n, a);
-  const int split = blockIdx.x;
-  if (split >= P.nsplit) return;
-
-  float qf[ND][VE], acc[ND][VE];
-  int dim[ND];  // this lane's dims, clamped into the row (their q is zero, they store nothing)
-  bool dvalid[ND];
-  const T* qp = reinterpret_cast<const T*>(a.d.q) + qrow * a.d.q_row + (int64_t)head * a.d.q_head;
-#pragma unroll
-  for (int j = 0; j < ND; ++j) {
-    const int d0 = (j * LPT + dg) * VE;
-    dvalid[j] = d0 < a.d.head_dim;
-    dim[j] = dvalid[j] ? d0 : 0;
-#pragma unroll
-    for (int i = 0; i < VE; ++i) {
-      qf[j][i] = dvalid[j] ? to_f32(qp[dim[j] + i]) * a.d.scale_log2 : 0.f;
-      acc[j][i] = 0.f;
+  WalkQ8 walk;
+  q8_start(a, first, walk);
+  ItemQ8 it;
+  while (q8_next(a, step, walk, it)) {
+    const int n = it.n, split = it.split;
+    T* out = reinterpret_cast<T*>(a.d.out) + it.qrow * a.d.o_row + (int64_t)head * a.d.o_head;
+    if (n <= 0) {
+      if (n == 0 && split == 0)
+        for (int d = lane; d < a.d.head_dim; d += 64) out[d] = from_f32<T>(0.f);
+      continue;
     }
-  }
-  const uint8_t* kbase = reinterpret_cast<const uint8_t*>(a.d.k) + (int64_t)kvh * a.d.k_head;
-  const uint8_t* vbase = reinterpret_cast<const uint8_t*>(a.d.v) + (int64_t)kvh * a.d.v_head;
-  const uint8_t* sbase = a.scales + (int64_t)kvh * a.s_head;
-  const int32_t* table = a.d.tables + trow * a.d.table_stride;
-  const int s0 = P.first + split * P.bps, s1 = min(s0 + P.bps, P.first + P.pages);
-  float m = -INFINITY, l = 0.f;
+    const PartitionQ8 P = partition_q8(n, a);
+    if (split >= P.nsplit) continue;
 
-  for (int seg = s0; seg < s1; seg += 64) {
-    // Up to 64 page ids and their scales, one page a lane.
-    const int seg1 = min(s1, seg + 64);
-    const int blk = seg + lane < seg1 ? pool_block(table[seg + lane], a) : 0;
-    const uint32_t ex = q8_exponents(sbase + (int64_t)blk * a.s_block);
-    // (int64: the last page's end may lie past 2^31 tokens)
-    const int tb = max(P.start, seg * a.d.block_size);
-    const int te = (int)min((int64_t)n, (int64_t)seg1 * a.d.block_size);
-    for (int left = te - tb; left > 0; left -= CH) {
-      const int p0 = te - left;
-      raw_t kr[U][ND], vr[U][ND];
-      float ks[U], vs[U];
+    float qf[ND][VE], acc[ND][VE];
+    int dim[ND];  // this lane's dims, clamped into the row (their q is zero, they store nothing)
+    bool dvalid[ND];
+    const T* qp = reinterpret_cast<const T*>(a.d.q) + it.qrow * a.d.q_row + (int64_t)head * a.d.q_head;
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        // Positions past the end read the last token again (and are masked).
-        const int pos = left > u * TPL + tg ? p0 + u * TPL + tg : te - 1;
-        int page, off;
-        if (a.d.bs_shift >= 0) {
-          page = pos >> a.d.bs_shift;
-          off = pos & (a.d.block_size - 1);
-        } else {
-          page = pos / a.d.block_size;
-          off = pos - page * a.d.block_size;
-        }
-        const int64_t b = shfl_i32(blk, page - seg);
-        const uint32_t e = (uint32_t)shfl_i32((int)ex, page - seg);
-        ks[u] = q8_scale(e & 255);
-        vs[u] = q8_scale(e >> 8);
+    for (int j = 0; j < ND; ++j) {
+      const int d0 = (j * LPT + dg) * VE;
+      dvalid[j] = d0 < a.d.head_dim;
+      dim[j] = dvalid[j] ? d0 : 0;
 #pragma unroll
-        for (int j = 0; j < ND; ++j) {
-          kr[u][j] = __builtin_nontemporal_load(reinterpret_cast<const raw_t*>(
-              kbase + b * a.d.k_block + (int64_t)off * a.d.k_token + dim[j]));
-          vr[u][j] = __builtin_nontemporal_load(reinterpret_cast<const raw_t*>(
-              vbase + b * a.d.v_block + (int64_t)off * a.d.v_token + dim[j]));
-        }
+      for (int i = 0; i < VE; ++i) {
+        qf[j][i] = dvalid[j] ? to_f32(qp[dim[j] + i]) * a.d.scale_log2 : 0.f;
+        acc[j][i] = 0.f;
       }
-      float sc[U], mx = m;
+    }
+    const uint8_t* kbase = reinterpret_cast<const uint8_t*>(a.d.k) + (int64_t)kvh * a.d.k_head;
+    const uint8_t* vbase = reinterpret_cast<const uint8_t*>(a.d.v) + (int64_t)kvh * a.d.v_head;
+    const uint8_t* sbase = a.scales + (int64_t)kvh * a.s_head;
+    const int32_t* table = a.d.tables + it.trow * a.d.table_stride;
+    const int s0 = P.first + split * P.bps, s1 = min(s0 + P.bps, P.first + P.pages);
+    float m = -INFINITY, l = 0.f;
+
+    for (int seg = s0; seg < s1; seg += 64) {
+      // Up to 64 page ids and their scales, one page a lane.
+      const int seg1 = min(s1, seg + 64);
+      const int blk = seg + lane < seg1 ? pool_block(table[seg + lane], a) : 0;
+      const uint32_t ex = q8_exponents(sbase + (int64_t)blk * a.s_block);
+      // (int64: the last page's end may lie past 2^31 tokens)
+      const int tb = max(P.start, seg * a.d.block_size);
+      const int te = (int)min((int64_t)n, (int64_t)seg1 * a.d.block_size);
+      for (int left = te - tb; left > 0; left -= CH) {
+        const int p0 = te - left;
+        raw_t kr[U][ND], vr[U][ND];
+        float ks[U], vs[U];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        float d = 0.f;
+        for (int u = 0; u < U; ++u) {
+          // Positions past the end read the last token again (and are masked).
+          const int pos = left > u * TPL + tg ? p0 + u * TPL + tg : te - 1;
+          int page, off;
+          if (a.d.bs_shift >= 0) {
+            page = pos >> a.d.bs_shift;
+            off = pos & (a.d.block_size - 1);
+          } else {
+            page = pos / a.d.block_size;
+            off = pos - page * a.d.block_size;
+          }
+          const int64_t b = shfl_i32(blk, page - seg);
+          const uint32_t e = (uint32_t)shfl_i32((int)ex, page - seg);
+          ks[u] = q8_scale(e & 255);
+          vs[u] = q8_scale(e >> 8);
 #pragma unroll
-        for (int j = 0; j < ND; ++j) {
-          float x[VE];
-          q8_values<VE>(kr[u][j], x);
-#pragma unroll
-          for (int i = 0; i < VE; ++i) d = fmaf(qf[j][i], x[i], d);
+          for (int j = 0; j < ND; ++j) {
+            kr[u][j] = __builtin_nontemporal_load(reinterpret_cast<const raw_t*>(
+                kbase + b * a.d.k_block + (int64_t)off * a.d.k_token + dim[j]));
+            vr[u][j] = __builtin_nontemporal_load(reinterpret_cast<const raw_t*>(
+                vbase + b * a.d.v_block + (int64_t)off * a.d.v_token + dim[j]));
+          }
         }
-        d = group_sum<LPT>(d) * ks[u];
-        sc[u] = left > u * TPL + tg ? d : -INFINITY;
-        mx = fmaxf(mx, sc[u]);
+        float sc[U], mx = m;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          float d = 0.f;
+#pragma unroll
+          for (int j = 0; j < ND; ++j) {
+            float x[VE];
+            q8_values<VE>(kr[u][j], x);
+#pragma unroll
+            for (int i = 0; i < VE; ++i) d = fmaf(qf[j][i], x[i], d);
+          }
+          d = group_sum<LPT>(d) * ks[u];
+          sc[u] = left > u * TPL + tg ? d : -INFINITY;
+          mx = fmaxf(mx, sc[u]);
+        }
+        const float safe = mx == -INFINITY ? 0.f : mx;
+        const float corr = fast_exp2(m - safe);
+        l *= corr;
+#pragma unroll
+        for (int j = 0; j < ND; ++j)
+#pragma unroll
+          for (int i = 0; i < VE; ++i) acc[j][i] *= corr;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const float p = fast_exp2(sc[u] - safe);
+          l += p;
+          const float w = p * vs[u];
+          // A masked token's weight is 0, and its value must not matter (0 * NaN).
+          const bool seen = left > u * TPL + tg;
+#pragma unroll
+          for (int j = 0; j < ND; ++j) {
+            float x[VE];
+            q8_values<VE>(vr[u][j], x);
+#pragma unroll
+            for (int i = 0; i < VE; ++i) acc[j][i] = seen ? fmaf(w, x[i], acc[j][i]) : acc[j][i];
+          }
+        }
+        m = mx;
       }
-      const float safe = mx == -INFINITY ? 0.f : mx;
-      const float corr = fast_exp2(m - safe);
-      l *= corr;
+    }
+    // Merge the token groups' states.
+    const float M = cross_group_max<LPT>(m);
+    // (l is 0 only where the group saw no token: a NaN score leaves m at -inf too)
+    const float w = l == 0.f ? 0.f : fast_exp2(m - M);
+    const float L = cross_group_sum<LPT>(l * w);
+#pragma unroll
+    for (int j = 0; j < ND; ++j)
+#pragma unroll
+      for (int i = 0; i < VE; ++i) acc[j][i] = cross_group_sum<LPT>(acc[j][i] * w);
+    if (tg != 0) continue;
+    if (P.nsplit == 1) {
+      const float inv = 1.f / L;
 #pragma unroll
       for (int j = 0; j < ND; ++j)
 #pragma unroll
-        for (int i = 0; i < VE; ++i) acc[j][i] *= corr;
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const float p = fast_exp2(sc[u] - safe);
-        l += p;
-        const float w = p * vs[u];
-        // A masked token's weight is 0, and its value must not matter (0 * NaN).
-        const bool seen = left > u * TPL + tg;
-#pragma unroll
-        for (int j = 0; j < ND; ++j) {
-          float x[VE];
-          q8_values<VE>(vr[u][j], x);
-#pragma unroll
-          for (int i = 0; i < VE; ++i) acc[j][i] = seen ? fmaf(w, x[i], acc[j][i]) : acc[j][i];
-        }
-      }
-      m = mx;
+        for (int i = 0; i < VE; ++i)
+          if (dvalid[j]) out[dim[j] + i] = from_f32<T>(acc[j][i] * inv);
+      continue;
     }
-  }
-  // Merge the token groups' states.
-  const float M = cross_group_max<LPT>(m);
-  // (l is 0 only where the group saw no token: a NaN score leaves m at -inf too)
-  const float w = l == 0.f ? 0.f : fast_exp2(m - M);
-  const float L = cross_group_sum<LPT>(l * w);
-#pragma unroll
-  for (int j = 0; j < ND; ++j)
-#pragma unroll
-    for (int i = 0; i < VE; ++i) acc[j][i] = cross_group_sum<LPT>(acc[j][i] * w);
-  if (tg != 0) return;
-  if (P.nsplit == 1) {
-    const float inv = 1.f / L;
+    const int64_t idx = (it.row * a.d.q_heads + head) * a.slots + split;
+    if (dg == 0) {
+      a.d.part_ml[idx * 2] = M;
+      a.d.part_ml[idx * 2 + 1] = L;
+    }
+    float* dst = a.d.part_acc + idx * a.d.head_dim;
 #pragma unroll
     for (int j = 0; j < ND; ++j)
 #pragma unroll
       for (int i = 0; i < VE; ++i)
-        if (dvalid[j]) out[dim[j] + i] = from_f32<T>(acc[j][i] * inv);
-    return;
+        if (dvalid[j]) dst[dim[j] + i] = acc[j][i];
   }
-  const int64_t idx = (row * a.d.q_heads + head) * a.slots + split;
-  if (dg == 0) {
-    a.d.part_ml[idx * 2] = M;
-    a.d.part_ml[idx * 2 + 1] = L;
-  }
-  float* dst = a.d.part_acc + idx * a.d.head_dim;
-#pragma unroll
-  for (int j = 0; j < ND; ++j)
-#pragma unroll
-    for (int i = 0; i < VE; ++i)
-      if (dvalid[j]) dst[dim[j] + i] = acc[j][i];
 }
 
 // ------------------------------------------------ 16-bit queries on MFMA
-// One wave per (run of splits, KV head, row) serves up to 16 q heads of the KV head (the
+// One wave per (split, KV head, row) serves up to 16 q heads of the KV head (the
 // columns of v_mfma_f32_16x16x32; groups of more take several waves):
 //  * K and V come in chunks of 32 tokens straight into a ring of kStages wave-private
-//    LDS stages, kStages - 1 chunks ahead and across the splits of the run: no registers
-//    are held by loads in flight and no barrier is needed. One load instruction covers
+//    LDS stages, kStages - 1 chunks ahead: no registers are held by loads in flight and no
+//    barrier is needed. One load instruction covers
 //    RPI whole rows; the block size is a power of two of at least 16, so 16-token steps
 //    lie in one page and take one (scalar) address.
 //  * S^T = K Q^T per 16 tokens: bytes are converted to the query's type (exact), 16 a
@@ -410,8 +392,8 @@ __global__ __launch_bounds__(64) void paged_decode_q8_mfma_kernel(DecodeQ8Args a
   const int col = lane & 15, grp = lane >> 4;
   const int bs = a.d.block_size, sh = a.d.bs_shift;
 
-  const uint32_t share = blockIdx.x / (uint32_t)a.units;
-  const int unit = (int)(blockIdx.x - share * (uint32_t)a.units);
+  const uint32_t first = blockIdx.x / (uint32_t)a.units, next = gridDim.x / (uint32_t)a.units;
+  const int unit = (int)(blockIdx.x - first * (uint32_t)a.units);
   const int kvh = a.tiles == 1 ? unit : unit / a.tiles;
   const int head0 = kvh * a.d.group + (unit - kvh * a.tiles) * 16;
   const int heads = min(16, (kvh + 1) * a.d.group - head0);
@@ -442,10 +424,10 @@ __global__ __launch_bounds__(64) void paged_decode_q8_mfma_kernel(DecodeQ8Args a
   for (int t = 0; t < DT; ++t)
     voff[t] = lds0 + kChunk * D + vrow * D + ((16 * q8_swizzle<D>(vrow)) ^ (16 * t)) + 8 * (col & 1);
 
-  ShareQ8 mine;
-  q8_share(a, share, gridDim.x / (uint32_t)a.units, mine);
+  WalkQ8 walk;
+  q8_start(a, first, walk);
   ItemQ8 it;
-  while (q8_next(a, mine, it)) {
+  while (q8_next(a, next, walk, it)) {
     const int n = it.n;
     T* out = reinterpret_cast<T*>(a.d.out) + it.qrow * a.d.o_row + (int64_t)(head0 + col) * a.d.o_head + 4 * grp;
     if (n <= 0) {
@@ -458,7 +440,7 @@ __global__ __launch_bounds__(64) void paged_decode_q8_mfma_kernel(DecodeQ8Args a
     const PartitionQ8 P = partition_q8(n, a);
     if (it.split >= P.nsplit) continue;
     const int s0 = P.first + it.split * P.bps;
-    const int s1 = min(s0 + it.splits * P.bps, P.first + P.pages);
+    const int s1 = min(s0 + P.bps, P.first + P.pages);
     const int32_t* table = a.d.tables + it.trow * a.d.table_stride;
     // The first page ids travel with the queries.
     int ids = s0 + lane < min(s1, s0 + kSegment) ? table[s0 + lane] : 0;
@@ -481,34 +463,6 @@ __global__ __launch_bounds__(64) void paged_decode_q8_mfma_kernel(DecodeQ8Args a
     f32x4_t acc[DT];
 #pragma unroll
     for (int t = 0; t < DT; ++t) acc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    int split = it.split;
-    // The end of a split: its partial (or the row's output), and a fresh state.
-    auto flush = [&]() __attribute__((always_inline)) {
-      lsum += shfl_xor_f32(lsum, 16);
-      lsum += shfl_xor_f32(lsum, 32);
-      if (hcol && P.nsplit == 1) {
-        const float inv = 1.f / lsum;
-#pragma unroll
-        for (int t = 0; t < DT; ++t)
-          *reinterpret_cast<u32x2_t*>(out + 16 * t) =
-              u32x2_t{pack2<T>(acc[t][0] * inv, acc[t][1] * inv), pack2<T>(acc[t][2] * inv, acc[t][3] * inv)};
-      } else if (hcol) {
-        const int64_t idx = (it.row * a.d.q_heads + head0 + col) * a.slots + split;
-        if (grp == 0) {
-          a.d.part_ml[idx * 2] = m;
-          a.d.part_ml[idx * 2 + 1] = lsum;
-        }
-        float* dst = a.d.part_acc + idx * D + 4 * grp;
-#pragma unroll
-        for (int t = 0; t < DT; ++t) *reinterpret_cast<f32x4_t*>(dst + 16 * t) = acc[t];
-      }
-      ++split;
-      m = -1e30f;
-      lsum = 0.f;
-#pragma unroll
-      for (int t = 0; t < DT; ++t) acc[t] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    };
-
     for (int seg = s0; seg < s1; seg += kSegment) {
       const int seg1 = min(s1, seg + kSegment);
       if (seg > s0) ids = seg + lane < seg1 ? table[seg + lane] : 0;
@@ -523,8 +477,6 @@ __global__ __launch_bounds__(64) void paged_decode_q8_mfma_kernel(DecodeQ8Args a
       const int te = (int)min((int64_t)n, (int64_t)seg1 << sh);
       // Chunk j holds tokens t0 + 32 j ..; those before the window's are not read.
       const int j0 = (tb - t0) / kChunk, j1 = (te - t0 + kChunk - 1) / kChunk;
-      // Chunks per split (one split longer than a segment is flushed after the last).
-      const int per = P.bps > kSegment ? INT32_MAX : (P.bps << sh) / kChunk;
 
       auto load = [&](int j, auto st_c) __attribute__((always_inline)) {
         constexpr int st = decltype(st_c)::value;
@@ -636,34 +588,18 @@ __global__ __launch_bounds__(64) void paged_decode_q8_mfma_kernel(DecodeQ8Args a
           acc[t] = MfmaQ8<T>::run(MfmaQ8<T>::widen(x[0], x[1], vs[0], vs[1]), pop, acc[t]);
         }
       };
-      // Step j: chunk j has landed (only the loads of later chunks, and a flush's stores,
-      // may be in flight); the stage of j - 1, whose reads have returned, takes chunk
-      // j + kStages - 1.
-      bool flushed = false;
-      int left = per - j0;  // chunks to the split's end (j0 > 0 only in the row's first)
+      // Step j: chunk j has landed (only the loads of later chunks may be in flight); the
+      // stage of j - 1, whose reads have returned, takes chunk j + kStages - 1.
       auto step = [&](int j, auto now_c) __attribute__((always_inline)) {
         constexpr int now = decltype(now_c)::value;
-        // A flush in the last step put at least DT stores behind the loads of j and j + 1.
         const int later = min(kStages - 2, j1 - 1 - j);
-        if (flushed) {
-          if (kStages > 3 && later == 2) wait_loads<4 * NI + DT>();
-          else if (kStages > 2 && later == 1) wait_loads<2 * NI + DT>();
-          else wait_loads<DT>();
-        } else {
-          if (kStages > 3 && later == 2) wait_loads<4 * NI>();
-          else if (kStages > 2 && later == 1) wait_loads<2 * NI>();
-          else wait_loads<0>();
-        }
-        flushed = false;
+        if (kStages > 3 && later == 2) wait_loads<4 * NI>();
+        else if (kStages > 2 && later == 1) wait_loads<2 * NI>();
+        else wait_loads<0>();
         if (j == j0) scales();
         if (j + kStages - 1 < j1) load(j + kStages - 1, std::integral_constant<int, (now + kStages - 1) % kStages>{});
         attend(j, now_c);
         wait_lds();
-        if (--left == 0) {
-          flush();
-          left = per;
-          flushed = true;
-        }
       };
       static_assert(kStages >= 2 && kStages <= 4, "the waits above");
       auto each_stage = [&](auto f) __attribute__((always_inline)) {
@@ -680,7 +616,25 @@ __global__ __launch_bounds__(64) void paged_decode_q8_mfma_kernel(DecodeQ8Args a
           if (j + decltype(st)::value < j1) step(j + decltype(st)::value, st);
         });
     }
-    if (split < it.split + it.splits) flush();  // the row's last split, or a long one
+    lsum += shfl_xor_f32(lsum, 16);
+    lsum += shfl_xor_f32(lsum, 32);
+    if (!hcol) continue;
+    if (P.nsplit == 1) {
+      const float inv = 1.f / lsum;
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+        *reinterpret_cast<u32x2_t*>(out + 16 * t) =
+            u32x2_t{pack2<T>(acc[t][0] * inv, acc[t][1] * inv), pack2<T>(acc[t][2] * inv, acc[t][3] * inv)};
+      continue;
+    }
+    const int64_t idx = (it.row * a.d.q_heads + head0 + col) * a.slots + it.split;
+    if (grp == 0) {
+      a.d.part_ml[idx * 2] = m;
+      a.d.part_ml[idx * 2 + 1] = lsum;
+    }
+    float* dst = a.d.part_acc + idx * D + 4 * grp;
+#pragma unroll
+    for (int t = 0; t < DT; ++t) *reinterpret_cast<f32x4_t*>(dst + 16 * t) = acc[t];
   }
 }
 
@@ -744,17 +698,17 @@ __global__ __launch_bounds__(256) void merge_q8_kernel(DecodeQ8Args a) {
 }
 
 template <typename T>
-void launch_valu(bool wide16, bool wide4, dim3 grid, hipStream_t s, const DecodeQ8Args& a) {
+void launch_valu(bool wide16, bool wide4, unsigned waves, hipStream_t s, const DecodeQ8Args& a) {
   if (wide16 && a.d.head_dim <= 64)
-    hipLaunchKernelGGL((paged_decode_q8_kernel<T, 16, 4, 1>), grid, dim3(64), 0, s, a);
+    hipLaunchKernelGGL((paged_decode_q8_kernel<T, 16, 4, 1>), dim3(waves), dim3(64), 0, s, a);
   else if (wide16 && a.d.head_dim <= 128)
-    hipLaunchKernelGGL((paged_decode_q8_kernel<T, 16, 8, 1>), grid, dim3(64), 0, s, a);
+    hipLaunchKernelGGL((paged_decode_q8_kernel<T, 16, 8, 1>), dim3(waves), dim3(64), 0, s, a);
   else if (wide16)
-    hipLaunchKernelGGL((paged_decode_q8_kernel<T, 16, 16, 1>), grid, dim3(64), 0, s, a);
+    hipLaunchKernelGGL((paged_decode_q8_kernel<T, 16, 16, 1>), dim3(waves), dim3(64), 0, s, a);
   else if (wide4)
-    hipLaunchKernelGGL((paged_decode_q8_kernel<T, 4, 64, 1>), grid, dim3(64), 0, s, a);
+    hipLaunchKernelGGL((paged_decode_q8_kernel<T, 4, 64, 1>), dim3(waves), dim3(64), 0, s, a);
   else
-    hipLaunchKernelGGL((paged_decode_q8_kernel<T, 1, 64, 4>), grid, dim3(64), 0, s, a);
+    hipLaunchKernelGGL((paged_decode_q8_kernel<T, 1, 64, 4>), dim3(waves), dim3(64), 0, s, a);
 }
 
 template <typename T, int ND>
@@ -883,38 +837,37 @@ int vrh_decode_rows_q8(const Q8Call& c, const int32_t* cu_q, int32_t num_seqs, i
                     c.o_row % 4 == 0 && c.o_head % 4 == 0 && (uintptr_t)c.q % 16 == 0 &&
                     (uintptr_t)c.out % 8 == 0 && c.s_block % 2 == 0 && c.s_head % 2 == 0 &&
                     (uintptr_t)c.scales % 2 == 0;
-  a.tiles = ceil_div(a.d.group, 16);
-  a.units = c.kv_heads * a.tiles;
+  a.tiles = mfma ? ceil_div(a.d.group, 16) : 1;
+  a.units = mfma ? c.kv_heads * a.tiles : c.q_heads;
   auto shift_of = [](int x) { return (x & (x - 1)) == 0 ? __builtin_ctz((unsigned)x) : -1; };
   a.min_shift = shift_of(a.d.min_bps);
   a.long_shift = shift_of(a.d.long_bps);
   a.split_unit = mfma ? std::max(1, kChunk / c.block_size) : 1;
-  a.compact = mfma && rows <= kCompactRows;
-  const int64_t per_row = mfma ? (int64_t)a.units * a.slots : 1;
+  a.compact = rows <= kCompactRows;
+  const int64_t per_row = (int64_t)a.units * a.slots;
   VRH_CHECK_ARG(per_row < (1ll << 30), "%s: too many heads", who);
   const int64_t kRowsPerLaunch = std::min<int64_t>(65535, (1ll << 31) / per_row - 1);
+  // Waves that are resident at once: by LDS, or of the VALU kernel by registers.
+  constexpr int64_t kCus = 256, kLds = 160 * 1024;
+  const int64_t resident = kCus * (mfma ? kLds / (kStages * 2 * kChunk * c.head_dim + 1024) : 12);
   for (int64_t first = 0; first < rows; first += kRowsPerLaunch) {
     a.d.row_base = first;
     const unsigned count = (unsigned)std::min<int64_t>(rows - first, kRowsPerLaunch);
-    // Waves of the matrix kernel that are resident at once, by LDS.
-    constexpr int64_t kCus = 256, kLds = 160 * 1024;
-    const int64_t resident = kCus * (kLds / (kStages * 2 * kChunk * c.head_dim + 1024)) / a.units * a.units;
-    const int64_t waves = a.compact ? std::min<int64_t>(count * per_row, std::max<int64_t>(kRounds * resident, a.units))
-                                    : count * per_row;
-    const dim3 grid((unsigned)a.slots, (unsigned)c.q_heads, count);
+    int64_t waves = count * per_row;
+    if (a.compact) waves = std::min(waves, std::max<int64_t>(1, resident / a.units) * a.units);
     switch (c.dtype) {
       case VRH_DTYPE_F32:
-        launch_valu<float>(cache_aligned(16), cache_aligned(4), grid, s, a);
+        launch_valu<float>(cache_aligned(16), cache_aligned(4), (unsigned)waves, s, a);
         if (a.slots > 1) launch_merge_q8<float>(count, s, a);
         break;
       case VRH_DTYPE_F16:
         if (mfma) launch_mfma_q8<f16_t>((unsigned)waves, s, a);
-        else launch_valu<f16_t>(cache_aligned(16), cache_aligned(4), grid, s, a);
+        else launch_valu<f16_t>(cache_aligned(16), cache_aligned(4), (unsigned)waves, s, a);
         if (a.slots > 1) launch_merge_q8<f16_t>(count, s, a);
         break;
       default:
         if (mfma) launch_mfma_q8<bf16_t>((unsigned)waves, s, a);
-        else launch_valu<bf16_t>(cache_aligned(16), cache_aligned(4), grid, s, a);
+        else launch_valu<bf16_t>(cache_aligned(16), cache_aligned(4), (unsigned)waves, s, a);
         if (a.slots > 1) launch_merge_q8<bf16_t>(count, s, a);
     }
   }
