@@ -21,7 +21,7 @@ namespace {
 // 113 us with splits of 128 tokens throughout, 107 with 256; 512 no better. Short rows
 // are what few waves have: one row of 300 tokens in three splits.
 constexpr int kSplitTokens = 128;
-constexpr int kLongTokens = 256;
+constexpr int kLongTokens = 256;  // (37 float16 rows, 32 over 8 heads: 48 us, 61 with 128, 55 with 512)
 constexpr int kShortTokens = 2048;
 constexpr int kMaxSplitsQ8 = 64;  // a lane each in the merge
 
@@ -340,8 +340,14 @@ __global__ __launch_bounds__(64) void paged_decode_q8_kernel(DecodeQ8Args a) {
 //    conversion applies the page's scale (exact in bf16; in f16 see v_scale).
 //  * A row of LDS is D bytes of 16-byte chunks, chunk c of row r stored at slot
 //    c ^ swizzle(r), so that both readers spread over all banks.
+// A stage is 8 KiB at head_dim 128: two of them leave nine waves to a CU, more than two to
+// a SIMD, and it is other waves that cover a chunk's chain of LDS reads, MFMAs and
+// exponentials (about 1800 cycles). Three stages and six waves: 64 rows of 512-4096 tokens
+// (16 x 128 heads) 112 us instead of 110, 37 float16 rows of 32 over 8 heads 51 instead of
+// 48, 24 rows with a window of 1024 23.6 instead of 20.4. Without the arithmetic those 64
+// rows take 101 us (6.0 TB/s), without the loads 75.
 constexpr int kChunk = 32;  // tokens per stage
-constexpr int kStages = 3;
+constexpr int kStages = 2;
 
 typedef __attribute__((ext_vector_type(4))) float f32x4_t;
 typedef __attribute__((ext_vector_type(4))) uint32_t u32x4_t;

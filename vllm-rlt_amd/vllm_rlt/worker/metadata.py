@@ -24,6 +24,7 @@ from dataclasses import dataclass
 import torch
 
 from vllm_rlt.attention.metadata import AttentionRows, plan_attention_metadata
+from vllm_rlt.kernels.hip_attention import sequence_metadata
 
 
 @dataclass(frozen=True, eq=False)
@@ -140,8 +141,6 @@ def sequence_kv_metadata(tables, table_rows, context_lengths, query_lengths, *, 
     of which the last ``query_lengths[r]`` are new. ``tokens`` and ``width`` are the step's
     (bucketed) token count and table width, known on the host; ``max_seqlen_q`` bounds the query
     lengths (``tokens`` without it). Tokens behind the last request's have ``write_mask`` False."""
-    from vllm_rlt.kernels.hip_attention import sequence_metadata
-
     if isinstance(block_size, bool) or not isinstance(block_size, int) or block_size <= 0:
         raise ValueError("block_size must be a positive integer")
     positions, blocks, offsets, mask, out_tables, lengths, cu = sequence_metadata(
