@@ -421,6 +421,28 @@ def test_prefill(gpu, dtype, hq, hkv, dim, bs, order, lengths, counts):
         check_attention(got[rows], *want, dtype, dim, n)
 
 
+@pytest.mark.parametrize("dtype,dim,bs", [(torch.bfloat16, 128, 16), (torch.float16, 64, 16),
+                                          (torch.float16, 128, 32), (torch.bfloat16, 96, 16)])
+def test_prefill_of_more_pages_than_are_staged_at_once(gpu, dtype, dim, bs):
+    """Pages and their scales are staged 512 at a time; with more than 64 sequences no tile is split,
+    so that a tile's keys run past a first and a second such segment."""
+    from vllm_rlt.kernels.hip_attention_q8 import paged_prefill_attention_q8
+
+    rng = np.random.default_rng(8)
+    lengths = [1040 * bs - 7, 521 * bs + 3] + [1] * 64
+    counts = [70, 33] + [1] * 64
+    tables, blocks = tables_of(rng, lengths, bs)
+    layer = Layer(gpu, blocks, bs, 1, dim, seed=2)
+    cu = np.concatenate([[0], np.cumsum(counts)])
+    q = torch.randn((int(cu[-1]), 2, dim), generator=torch.Generator().manual_seed(4)).to(dtype)
+    got = paged_prefill_attention_q8(q.to(gpu), *layer.args, ints(tables, gpu), ints(lengths, gpu),
+                                     ints(cu, gpu), max(counts))
+    for s, (n, c) in enumerate(zip(lengths, counts)):
+        rows = slice(int(cu[s]), int(cu[s + 1]))
+        want = ref.attend(to64(q[rows]), *layer.context(tables[s], n), n - c)
+        check_attention(got[rows], *want, dtype, dim, n)
+
+
 @pytest.mark.parametrize("dtype,hq,hkv,dim", [(torch.bfloat16, 16, 16, 128), (torch.float16, 32, 8, 64),
                                               (torch.float32, 4, 2, 64), (torch.bfloat16, 4, 4, 96)])
 def test_short_packed_queries_equal_decode(gpu, dtype, hq, hkv, dim):

@@ -622,7 +622,9 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerEu, kWavesPerEu))) void paged_prefil
     const uint32_t kl = lds_offset(ks[stage]) + 1024 * wave;
     const uint32_t vl = lds_offset(vs[stage]) + 1024 * wave;
     const int k0 = j * kSB;
-    if (((min(k0 + kSB, end) - 1) >> a.bs_shift) >= tbl_base + kTableSeg) load_table(k0 >> a.bs_shift);
+    // (from sub-block j - 2 on: that and the next one still need their pages' scales)
+    if (((min(k0 + kSB, end) - 1) >> a.bs_shift) >= tbl_base + kTableSeg)
+      load_table((max(j - 2, j0) * kSB) >> a.bs_shift);
     if (kPow2 && a.uniform_pages && lane_off32 && k0 + kSB <= end) {
       // IR whole rows of one page per instruction: a scalar address.
       uint64_t off[NI];
