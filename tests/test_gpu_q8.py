@@ -351,6 +351,44 @@ def test_decode_of_one_very_long_row(gpu, dtype, bs, n):
         check_attention(got, *want, dtype, 64, n)
 
 
+def test_decode_of_more_waves_than_a_launch_holds(gpu):
+    """2200 rows x 512 heads x 64 split slots: the rows take several launches."""
+    from vllm_rlt.kernels.hip_attention_q8 import paged_attention_q8
+
+    rng = np.random.default_rng(3)
+    tables, blocks = tables_of(rng, [40], 16, width=1024)
+    layer = Layer(gpu, blocks, 16, 1, 4)
+    lengths = rng.integers(0, 41, 2200)
+    lengths[[0, -1]] = 40, 39
+    q = torch.randn((2200, 512, 4), generator=torch.Generator().manual_seed(4)).to(gpu)
+    got = paged_attention_q8(q, *layer.args, ints(tables, gpu).expand(2200, -1).contiguous(), ints(lengths, gpu))
+    for r in (0, 1, 1000, 2046, 2047, 2048, 2199):
+        n = int(lengths[r])
+        if n == 0:
+            assert not got[r].any()
+            continue
+        want = ref.attend(to64(q[r : r + 1]), *layer.context(tables[0], n), n - 1)
+        check_attention(got[r : r + 1], *want, torch.float32, 4, n)
+
+
+def test_append_and_read_of_more_pages_than_a_launch_holds(gpu):
+    """Pages of one token and one value that has four significant bits: all are exact."""
+    from vllm_rlt.kernels.hip_attention_q8 import kv_append_q8, kv_read_q8
+
+    pages = (1 << 23) + 1000
+    gen = torch.Generator(device=gpu).manual_seed(1)
+    k, v = (torch.randint(8, 16, (pages, 1, 1), generator=gen, device=gpu) *
+            2.0 ** torch.randint(-20, 20, (pages, 1, 1), generator=gen, device=gpu) for _ in range(2))
+    k, v = k.bfloat16(), v.bfloat16()
+    caches = [torch.zeros((pages, 1, 1, 1), dtype=torch.uint8, device=gpu).view(torch.float8_e4m3fn)
+              for _ in range(2)]
+    scales = torch.zeros((pages, 1, 2), dtype=torch.uint8, device=gpu)
+    tables = torch.randperm(pages, generator=gen, device=gpu).int()[None]
+    kv_append_q8(*caches, scales, k, v, tables, ints([pages], gpu), ints([0, pages], gpu))
+    got = kv_read_q8(*caches, scales, tables[0].long(), torch.bfloat16)
+    assert torch.equal(got[0].view(-1), k.view(-1)) and torch.equal(got[1].view(-1), v.view(-1))
+
+
 def test_decode_in_a_pool_past_32_bit_offsets(gpu):
     """Blocks more than 2^31 and 2^32 bytes into the cache."""
     from vllm_rlt.kernels.hip_attention_q8 import kv_append_q8, kv_read_q8, paged_attention_q8

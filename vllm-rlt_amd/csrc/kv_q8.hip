@@ -31,7 +31,7 @@ struct Q8AppendArgs {
   int64_t c_block, c_token, c_head;
   int64_t s_block, s_head;
   int64_t k_row, k_head, v_row, v_head;
-  int64_t num_seqs, total_q, num_blocks, table_stride;
+  int64_t num_seqs, total_q, num_blocks, table_stride, slot_base;
   int32_t heads, head_dim, block_size, table_width;
   int32_t shift;  // log2(vectors per head) or -1
 };
@@ -136,7 +136,7 @@ __global__ __launch_bounds__(256) void kv_append_q8_kernel(Q8AppendArgs a) {
   if (item >= 2 * a.heads) return;
   const int head = item >> 1, part = item & 1;
   Q8Slot at;
-  if (!q8_slot(a, blockIdx.x, at)) return;
+  if (!q8_slot(a, a.slot_base + blockIdx.x, at)) return;
   const int64_t row0 = at.row0, q = at.q, n = at.n;
   if (q <= 0 || n <= 0) return;
   // Positions before 0 or past the table take no row.
@@ -273,6 +273,8 @@ __global__ __launch_bounds__(256) void kv_read_q8_kernel(Q8ReadArgs a) {
   }
 }
 
+constexpr int64_t kMostPages = 1ll << 23;  // per launch: of 256 threads each, less than 2^32
+
 // Whether vectors of `ve` elements keep every access of a kernel aligned.
 bool aligned_vectors(int ve, int es, int64_t head_dim, std::initializer_list<int64_t> cache_strides,
                      std::initializer_list<int64_t> row_strides, std::initializer_list<const void*> caches,
@@ -318,7 +320,6 @@ extern "C" int vrh_kv_append_q8(int dtype, void* key_cache, void* value_cache, v
   VRH_CHECK_ARG(key_cache && value_cache && scales && k && v && block_tables && context_lengths,
                 "%s: null pointer", who);
   const int64_t slots = cu_seqlens_q ? total_q / block_size + 2 * num_seqs : num_seqs;
-  VRH_CHECK_ARG(slots < (1ll << 31), "%s: too many rows", who);
   Q8AppendArgs a;
   a.k_cache = (uint8_t*)key_cache;
   a.v_cache = (uint8_t*)value_cache;
@@ -351,19 +352,23 @@ extern "C" int vrh_kv_append_q8(int dtype, void* key_cache, void* value_cache, v
       {k_row_stride, k_head_stride, v_row_stride, v_head_stride}, {key_cache, value_cache}, {k, v});
   const int per_token = wide ? head_dim / ve : head_dim;
   a.shift = (per_token & (per_token - 1)) == 0 ? __builtin_ctz((unsigned)per_token) : -1;
-  const dim3 grid((unsigned)slots, (unsigned)ceil_div(2 * kv_heads, 4));
   hipStream_t s = (hipStream_t)stream;
-#define VRH_APPEND(T)                                                                          \
+  for (int64_t first = 0; first < slots; first += kMostPages) {
+    a.slot_base = first;
+    const dim3 grid((unsigned)(slots - first < kMostPages ? slots - first : kMostPages),
+                    (unsigned)ceil_div(2 * kv_heads, 4));
+#define VRH_APPEND(T)                                                                                 \
   if (wide) hipLaunchKernelGGL((kv_append_q8_kernel<T, 16 / sizeof(T)>), grid, dim3(256), 0, s, a); \
   else hipLaunchKernelGGL((kv_append_q8_kernel<T, 1>), grid, dim3(256), 0, s, a);
-  if (dtype == VRH_DTYPE_F32) {
-    VRH_APPEND(float)
-  } else if (dtype == VRH_DTYPE_F16) {
-    VRH_APPEND(f16_t)
-  } else {
-    VRH_APPEND(bf16_t)
-  }
+    if (dtype == VRH_DTYPE_F32) {
+      VRH_APPEND(float)
+    } else if (dtype == VRH_DTYPE_F16) {
+      VRH_APPEND(f16_t)
+    } else {
+      VRH_APPEND(bf16_t)
+    }
 #undef VRH_APPEND
+  }
   VRH_RETURN_LAUNCH(who);
 }
 
@@ -403,10 +408,9 @@ extern "C" int vrh_kv_read_q8(int dtype, void* out_k, void* out_v, const void* k
                                     {cache_block_stride, cache_token_stride, cache_head_stride}, {},
                                     {key_cache, value_cache}, {out_k, out_v});
   hipStream_t s = (hipStream_t)stream;
-  constexpr int64_t kMost = 1ll << 30;  // pages per launch
-  for (int64_t first = 0; first < num_pages; first += kMost) {
+  for (int64_t first = 0; first < num_pages; first += kMostPages) {
     a.page_base = first;
-    const dim3 grid((unsigned)(num_pages - first < kMost ? num_pages - first : kMost),
+    const dim3 grid((unsigned)(num_pages - first < kMostPages ? num_pages - first : kMostPages),
                     (unsigned)ceil_div(2 * kv_heads, 4));
 #define VRH_READ(T)                                                                     \
   if (wide) hipLaunchKernelGGL((kv_read_q8_kernel<T, 16>), grid, dim3(256), 0, s, a);   \

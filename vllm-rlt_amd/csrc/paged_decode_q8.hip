@@ -851,8 +851,10 @@ int vrh_decode_rows_q8(const Q8Call& c, const int32_t* cu_q, int32_t num_seqs, i
   a.split_unit = mfma ? std::max(1, kChunk / c.block_size) : 1;
   a.compact = rows <= kCompactRows;
   const int64_t per_row = (int64_t)a.units * a.slots;
-  VRH_CHECK_ARG(per_row < (1ll << 30), "%s: too many heads", who);
-  const int64_t kRowsPerLaunch = std::min<int64_t>(65535, (1ll << 31) / per_row - 1);
+  // A launch has less than 2^32 threads (65535 heads of kMaxSplitsQ8 splits at most, so at
+  // least one row); the waves that share the splits are fewer, and walk all rows.
+  const int64_t kRowsPerLaunch =
+      a.compact ? rows : std::min<int64_t>(65535, ((1ll << 26) - 1) / per_row);
   // Waves that are resident at once: by LDS, or of the VALU kernel by registers.
   constexpr int64_t kCus = 256, kLds = 160 * 1024;
   const int64_t resident = kCus * (mfma ? kLds / (kStages * 2 * kChunk * c.head_dim + 1024) : 12);
