@@ -326,7 +326,7 @@ def test_refusals(gpu):
     good = (tables, ints([0, 1], gpu, torch.int64), lengths, ints([1, 1], gpu), 16)
     sequence_metadata(*good, tokens=2, out_width=1)
     for at, bad, message in ((0, tables.long(), "int32"), (1, lengths, "int64"), (2, lengths[:1], "equal lengths"),
-                             (4, 0, "page")):
+                             (4, 0, "page"), (4, (1 << 32) + 16, "32-bit")):
         with pytest.raises(ValueError, match=message):
             sequence_metadata(*[bad if i == at else x for i, x in enumerate(good)], tokens=2, out_width=1)
     with pytest.raises(ValueError, match="tokens"):

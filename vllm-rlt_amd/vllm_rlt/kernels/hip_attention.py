@@ -607,8 +607,8 @@ def sequence_metadata(tables, table_rows, context_lengths, query_lengths, page, 
         raise ValueError("table_rows, context_lengths and query_lengths must have equal lengths")
     if tables.shape[1] > 1 and tables.stride(1) != 1:
         raise ValueError("tables rows must be contiguous")
-    if page < 1 or tokens < 0 or out_width < 0:
-        raise ValueError("page must be positive, tokens and out_width nonnegative")
+    if not 0 < page < 1 << 31 or not 0 <= tokens < 1 << 31 or not 0 <= out_width < 1 << 31:
+        raise ValueError("page must be positive, tokens and out_width nonnegative, all 32-bit")
     wide = torch.empty((3, tokens), dtype=torch.int64, device=device)
     mask = torch.empty(tokens, dtype=torch.bool, device=device)
     block_tables = torch.empty((n, out_width), dtype=torch.int32, device=device)
