@@ -522,24 +522,41 @@ Metadata sequence_metadata(const at::Tensor& tables, const at::Tensor& rows_in,
   const c10::DeviceGuard guard(tables.device());
   const at::Tensor rows = rows_in.contiguous(), lengths = lengths_in.contiguous(),
                    counts = counts_in.contiguous();
-  // Outputs of the op itself: nothing here is for autograd to see.
-  const at::AutoDispatchBelowADInplaceOrView below;
-  const auto ints = tables.options();
-  const at::Tensor wide = at::empty({3, tokens}, ints.dtype(at::kLong));
-  at::Tensor mask = at::empty({tokens}, ints.dtype(at::kBool));
-  at::Tensor out_tables = at::empty({n, out_width}, ints);
-  const at::Tensor narrow = at::empty({2 * n + 1}, ints);
-  int64_t* w = wide.data_ptr<int64_t>();
-  int32_t* m = narrow.data_ptr<int32_t>();
+  TORCH_CHECK(tokens < (1ll << 31) && n < (1ll << 31), "too many tokens or requests");
+  // One allocation for the seven outputs, 64-byte aligned parts: four allocations and five
+  // views of them took as long on the host as the kernel does on the GPU.
+  int64_t bytes = 0;
+  auto part = [&](int64_t count, int64_t size) {
+    const int64_t at = bytes;
+    bytes += (count * size + 63) / 64 * 64;
+    return at;
+  };
+  const int64_t positions = part(tokens, 8), blocks = part(tokens, 8), offsets = part(tokens, 8);
+  const int64_t mask = part(tokens, 1), out_tables = part(n * out_width, 4);
+  const int64_t out_lengths = part(n, 4), cu = part(n + 1, 4);
+  const at::Tensor all = at::empty({bytes}, tables.options().dtype(at::kByte));
+  auto view = [&](int64_t at, at::ScalarType type, at::IntArrayRef sizes) {
+    at::Tensor t = at::detail::make_tensor<c10::TensorImpl>(
+        c10::Storage(all.storage()), c10::DispatchKeySet(c10::DispatchKey::CUDA), c10::scalarTypeToTypeMeta(type));
+    t.unsafeGetTensorImpl()->set_storage_offset((all.storage_offset() + at) / (int64_t)c10::elementSize(type));
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(sizes);
+    return t;
+  };
+  char* base = static_cast<char*>(all.data_ptr());
+  auto longs = [&](int64_t at) { return reinterpret_cast<int64_t*>(base + at); };
+  auto ints = [&](int64_t at) { return reinterpret_cast<int32_t*>(base + at); };
   check_rc(vrh_sequence_metadata(tables.data_ptr<int32_t>(), tables.size(0), tables.stride(0),
                                  rows.data_ptr<int64_t>(), lengths.data_ptr<int32_t>(),
-                                 counts.data_ptr<int32_t>(), w, w + tokens, w + 2 * tokens,
-                                 reinterpret_cast<uint8_t*>(mask.data_ptr<bool>()),
-                                 out_tables.data_ptr<int32_t>(), out_width, m, m + n, n, tokens,
+                                 counts.data_ptr<int32_t>(), longs(positions), longs(blocks),
+                                 longs(offsets), reinterpret_cast<uint8_t*>(base + mask),
+                                 ints(out_tables), out_width, ints(out_lengths), ints(cu), n, tokens,
                                  (int32_t)tables.size(1), (int32_t)out_width, (int32_t)page,
                                  stream_of(tables)),
            "vrh_sequence_metadata");
-  return {wide.select(0, 0), wide.select(0, 1), wide.select(0, 2), mask, out_tables, narrow.narrow(0, 0, n), narrow.narrow(0, n, n + 1)};
+  return {view(positions, at::kLong, {tokens}), view(blocks, at::kLong, {tokens}),
+          view(offsets, at::kLong, {tokens}), view(mask, at::kBool, {tokens}),
+          view(out_tables, at::kInt, {n, out_width}), view(out_lengths, at::kInt, {n}),
+          view(cu, at::kInt, {n + 1})};
 }
 
 }  // namespace

@@ -252,6 +252,11 @@ class QuantizedKVPool:
         self.key_store = torch.zeros(shape, dtype=torch.uint8, device=self.device)
         self.value_store = torch.zeros_like(self.key_store)
         self.scales = torch.zeros((*shape[:3], 2), dtype=torch.uint8, device=self.device)
+        # Seven view operations a layer cost more host time than a decode step's append takes.
+        self._layers = [
+            (*(store[:, i].transpose(1, 2).view(hip_q8.CACHE_DTYPE)
+               for store in (self.key_store, self.value_store)), self.scales[:, i])
+            for i in range(self.num_layers)]
 
     def layer(self, layer: int) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         """One layer's ``[blocks, block_size, kv_heads, head_dim]`` K and V and ``[blocks, kv_heads,
@@ -259,8 +264,7 @@ class QuantizedKVPool:
         if isinstance(layer, bool) or not isinstance(layer, Integral) \
                 or not 0 <= layer < self.num_layers:
             raise ValueError(f"layer must be in [0, {self.num_layers})")
-        return (*(store[:, layer].transpose(1, 2).view(hip_q8.CACHE_DTYPE)
-                  for store in (self.key_store, self.value_store)), self.scales[:, layer])
+        return self._layers[layer]
 
     def append(self, layer, k, v, block_tables, context_lengths, cu_seqlens_q=None) -> None:
         """Quantise the newest tokens of every sequence into its pages (``kv_append_q8``)."""
