@@ -25,12 +25,6 @@ struct Q8Call {
   int64_t s_block, s_head;
 };
 
-// Decode rows (the rows of cu_q / expand_e: see DecodeArgs). With one_split every row
-// is one split and needs no workspace.
-int vrh_decode_rows_q8(const Q8Call& c, const int32_t* cu_q, int32_t num_seqs, int32_t expand_e,
-                       int64_t rows, int32_t window, void* workspace, size_t workspace_bytes,
-                       bool one_split, hipStream_t s, const char* who);
-
 namespace vrh {
 
 struct DecodeQ8Args {
@@ -51,6 +45,113 @@ struct DecodeQ8Args {
 // mistake) reads some block instead of memory outside the pool.
 __device__ __forceinline__ int pool_block(int id, const DecodeQ8Args& a) {
   return (int)max((int64_t)0, min((int64_t)id, a.num_blocks - 1));
+}
+
+// Splits of rows of up to kShortTokens visible tokens and of longer ones, and the most
+// splits of a row. Long rows come in batches or are cut into many splits anyway, and a
+// split costs a wave's start and a partial: 64 rows of 512-4096 tokens (16 x 128 heads)
+// 113 us with splits of 128 tokens throughout, 107 with 256; 512 no better. Short rows
+// are what few waves have: one row of 300 tokens in three splits.
+constexpr int kSplitTokens = 128;
+constexpr int kLongTokens = 256;  // (37 float16 rows, 32 over 8 heads: 48 us, 61 with 128, 55 with 512)
+constexpr int kShortTokens = 2048;
+constexpr int kMaxSplitsQ8 = 64;  // a lane each in the merge
+
+struct PartitionQ8 {
+  int start;   // first visible token
+  int first;   // first page
+  int pages;   // pages touched
+  int bps;     // pages per split
+  int nsplit;
+};
+
+__device__ __forceinline__ PartitionQ8 partition_q8(int n, const DecodeQ8Args& a) {
+  PartitionQ8 p;
+  p.start = (a.d.window > 0 && n > a.d.window) ? n - a.d.window : 0;
+  if (a.d.bs_shift >= 0) {
+    p.first = p.start >> a.d.bs_shift;
+    p.pages = ((n - 1) >> a.d.bs_shift) + 1 - p.first;
+  } else {
+    p.first = p.start / a.d.block_size;
+    p.pages = (n - 1) / a.d.block_size + 1 - p.first;
+  }
+  // Fewer slots than the most splits: the table (or window) has no longer rows, or one
+  // split is asked for.
+  if (a.slots == 1) {
+    p.bps = (p.pages + a.split_unit - 1) & -a.split_unit;
+    p.nsplit = 1;
+  } else {
+    const bool longer = p.pages > a.d.short_pages;
+    const int shift = longer ? a.long_shift : a.min_shift;
+    if (shift >= 0 && p.pages <= kMaxSplitsQ8 << shift) {
+      p.bps = 1 << shift;  // (no division: a wave does this before its first load)
+      p.nsplit = (p.pages + p.bps - 1) >> shift;
+    } else {
+      p.bps = max(longer ? a.d.long_bps : a.d.min_bps, (p.pages + kMaxSplitsQ8 - 1) / kMaxSplitsQ8);
+      p.bps = (p.bps + a.split_unit - 1) & -a.split_unit;
+      p.nsplit = (int)((uint32_t)(p.pages + p.bps - 1) / (uint32_t)p.bps);
+    }
+  }
+  return p;
+}
+
+// The partials of a (row, q head), ND dims a lane: up to kGroup splits by one wave, in
+// split order with all loads in flight at once; more by WAVES waves, a group each, whose
+// sums are added in order (so that the result does not depend on WAVES).
+constexpr int kGroup = 16;
+// Workgroups of 4 waves: `block` of the ceil(q_heads * WAVES / 4) of a row.
+template <typename T, int ND, int WAVES>
+__device__ __forceinline__ void merge_q8(const DecodeQ8Args& a, int block, int64_t row) {
+  constexpr int kHeads = 4 / WAVES;  // of a workgroup
+  const int lane = threadIdx.x & 63;
+  const int wave = threadIdx.x >> 6;
+  const int head = block * kHeads + wave / WAVES;
+  const int group = wave % WAVES;
+  if (head >= a.d.q_heads) return;
+  int64_t trow, qrow;
+  const int n = row_length(row, a.d, &trow, &qrow);
+  if (n <= 0) return;
+  const PartitionQ8 P = partition_q8(n, a);
+  if (P.nsplit <= 1) return;
+  const int64_t idx = (row * a.d.q_heads + head) * a.slots;
+  const int s0 = kGroup * group;
+  const float* src = a.d.part_acc + (idx + s0) * a.d.head_dim;
+  float x[kGroup][ND];
+#pragma unroll
+  for (int u = 0; u < kGroup; ++u)
+#pragma unroll
+    for (int j = 0; j < ND; ++j) {
+      const int d = lane + 64 * j;
+      x[u][j] = s0 + u < P.nsplit && d < a.d.head_dim ? src[u * a.d.head_dim + d] : 0.f;
+    }
+  const float mi = lane < P.nsplit ? a.d.part_ml[(idx + lane) * 2] : -INFINITY;
+  const float li = lane < P.nsplit ? a.d.part_ml[(idx + lane) * 2 + 1] : 0.f;
+  const float M = wave_max(mi);
+  const float wi = lane < P.nsplit ? fast_exp2(mi - M) : 0.f;
+  const float inv = 1.f / wave_sum(wi * li);
+  float acc[ND] = {};
+#pragma unroll
+  for (int u = 0; u < kGroup; ++u) {
+    const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wi), s0 + u));
+    if (s0 + u < P.nsplit) {
+#pragma unroll
+      for (int j = 0; j < ND; ++j) acc[j] = fmaf(w, x[u][j], acc[j]);
+    }
+  }
+  if constexpr (WAVES > 1) {
+    __shared__ float sums[WAVES][ND][64];
+#pragma unroll
+    for (int j = 0; j < ND; ++j) sums[group][j][lane] = acc[j];
+    __syncthreads();
+    if (group > 0) return;
+    for (int g = 1; g * kGroup < P.nsplit; ++g)
+#pragma unroll
+      for (int j = 0; j < ND; ++j) acc[j] += sums[g][j][lane];
+  }
+  T* out = reinterpret_cast<T*>(a.d.out) + qrow * a.d.o_row + (int64_t)head * a.d.o_head;
+#pragma unroll
+  for (int j = 0; j < ND; ++j)
+    if (lane + 64 * j < a.d.head_dim) out[lane + 64 * j] = from_f32<T>(acc[j] * inv);
 }
 
 // Scale exponents of one (page, head): K's in bits 0-7, V's in bits 8-15.
@@ -174,3 +275,13 @@ __device__ __forceinline__ void wait_lds() {
 }
 
 }  // namespace vrh
+
+// Decode rows (the rows of cu_q / expand_e: see DecodeArgs). With one_split every row
+// is one split and needs no workspace. With `later`, rows that fit one launch may be left
+// unmerged: *later_blocks > 0 workgroups of 4 waves, block b running merge_q8 of block
+// b % B of row b / B, B = ceil(q_heads * WAVES / 4), are then the caller's to launch
+// (WAVES: 1 with up to kGroup slots, otherwise 4).
+int vrh_decode_rows_q8(const Q8Call& c, const int32_t* cu_q, int32_t num_seqs, int32_t expand_e,
+                       int64_t rows, int32_t window, void* workspace, size_t workspace_bytes,
+                       bool one_split, hipStream_t s, const char* who, vrh::DecodeQ8Args* later = nullptr,
+                       unsigned* later_blocks = nullptr);

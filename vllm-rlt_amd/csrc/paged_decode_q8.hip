@@ -15,54 +15,6 @@
 namespace vrh {
 namespace {
 
-// Splits of rows of up to kShortTokens visible tokens and of longer ones, and the most
-// splits of a row. Long rows come in batches or are cut into many splits anyway, and a
-// split costs a wave's start and a partial: 64 rows of 512-4096 tokens (16 x 128 heads)
-// 113 us with splits of 128 tokens throughout, 107 with 256; 512 no better. Short rows
-// are what few waves have: one row of 300 tokens in three splits.
-constexpr int kSplitTokens = 128;
-constexpr int kLongTokens = 256;  // (37 float16 rows, 32 over 8 heads: 48 us, 61 with 128, 55 with 512)
-constexpr int kShortTokens = 2048;
-constexpr int kMaxSplitsQ8 = 64;  // a lane each in the merge
-
-struct PartitionQ8 {
-  int start;   // first visible token
-  int first;   // first page
-  int pages;   // pages touched
-  int bps;     // pages per split
-  int nsplit;
-};
-
-__device__ __forceinline__ PartitionQ8 partition_q8(int n, const DecodeQ8Args& a) {
-  PartitionQ8 p;
-  p.start = (a.d.window > 0 && n > a.d.window) ? n - a.d.window : 0;
-  if (a.d.bs_shift >= 0) {
-    p.first = p.start >> a.d.bs_shift;
-    p.pages = ((n - 1) >> a.d.bs_shift) + 1 - p.first;
-  } else {
-    p.first = p.start / a.d.block_size;
-    p.pages = (n - 1) / a.d.block_size + 1 - p.first;
-  }
-  // Fewer slots than the most splits: the table (or window) has no longer rows, or one
-  // split is asked for.
-  if (a.slots == 1) {
-    p.bps = (p.pages + a.split_unit - 1) & -a.split_unit;
-    p.nsplit = 1;
-  } else {
-    const bool longer = p.pages > a.d.short_pages;
-    const int shift = longer ? a.long_shift : a.min_shift;
-    if (shift >= 0 && p.pages <= kMaxSplitsQ8 << shift) {
-      p.bps = 1 << shift;  // (no division: a wave does this before its first load)
-      p.nsplit = (p.pages + p.bps - 1) >> shift;
-    } else {
-      p.bps = max(longer ? a.d.long_bps : a.d.min_bps, (p.pages + kMaxSplitsQ8 - 1) / kMaxSplitsQ8);
-      p.bps = (p.bps + a.split_unit - 1) & -a.split_unit;
-      p.nsplit = (int)((uint32_t)(p.pages + p.bps - 1) / (uint32_t)p.bps);
-    }
-  }
-  return p;
-}
-
 __device__ __forceinline__ int page_of(int pos, const DecodeQ8Args& a) {
   return a.d.bs_shift >= 0 ? pos >> a.d.bs_shift : pos / a.d.block_size;
 }
@@ -644,63 +596,9 @@ __global__ __launch_bounds__(64) void paged_decode_q8_mfma_kernel(DecodeQ8Args a
   }
 }
 
-// The partials of a (row, q head), ND dims a lane: up to kGroup splits by one wave, in
-// split order with all loads in flight at once; more by WAVES waves, a group each, whose
-// sums are added in order (so that the result does not depend on WAVES).
-constexpr int kGroup = 16;
 template <typename T, int ND, int WAVES>
 __global__ __launch_bounds__(256) void merge_q8_kernel(DecodeQ8Args a) {
-  constexpr int kHeads = 4 / WAVES;  // of a workgroup
-  const int lane = threadIdx.x & 63;
-  const int wave = threadIdx.x >> 6;
-  const int head = blockIdx.x * kHeads + wave / WAVES;
-  const int group = wave % WAVES;
-  const int64_t row = a.d.row_base + blockIdx.y;
-  if (head >= a.d.q_heads) return;
-  int64_t trow, qrow;
-  const int n = row_length(row, a.d, &trow, &qrow);
-  if (n <= 0) return;
-  const PartitionQ8 P = partition_q8(n, a);
-  if (P.nsplit <= 1) return;
-  const int64_t idx = (row * a.d.q_heads + head) * a.slots;
-  const int s0 = kGroup * group;
-  const float* src = a.d.part_acc + (idx + s0) * a.d.head_dim;
-  float x[kGroup][ND];
-#pragma unroll
-  for (int u = 0; u < kGroup; ++u)
-#pragma unroll
-    for (int j = 0; j < ND; ++j) {
-      const int d = lane + 64 * j;
-      x[u][j] = s0 + u < P.nsplit && d < a.d.head_dim ? src[u * a.d.head_dim + d] : 0.f;
-    }
-  const float mi = lane < P.nsplit ? a.d.part_ml[(idx + lane) * 2] : -INFINITY;
-  const float li = lane < P.nsplit ? a.d.part_ml[(idx + lane) * 2 + 1] : 0.f;
-  const float M = wave_max(mi);
-  const float wi = lane < P.nsplit ? fast_exp2(mi - M) : 0.f;
-  const float inv = 1.f / wave_sum(wi * li);
-  float acc[ND] = {};
-#pragma unroll
-  for (int u = 0; u < kGroup; ++u) {
-    const float w = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wi), s0 + u));
-    if (s0 + u < P.nsplit) {
-#pragma unroll
-      for (int j = 0; j < ND; ++j) acc[j] = fmaf(w, x[u][j], acc[j]);
-    }
-  }
-  if constexpr (WAVES > 1) {
-    __shared__ float sums[WAVES][ND][64];
-#pragma unroll
-    for (int j = 0; j < ND; ++j) sums[group][j][lane] = acc[j];
-    __syncthreads();
-    if (group > 0) return;
-    for (int g = 1; g * kGroup < P.nsplit; ++g)
-#pragma unroll
-      for (int j = 0; j < ND; ++j) acc[j] += sums[g][j][lane];
-  }
-  T* out = reinterpret_cast<T*>(a.d.out) + qrow * a.d.o_row + (int64_t)head * a.d.o_head;
-#pragma unroll
-  for (int j = 0; j < ND; ++j)
-    if (lane + 64 * j < a.d.head_dim) out[lane + 64 * j] = from_f32<T>(acc[j] * inv);
+  merge_q8<T, ND, WAVES>(a, blockIdx.x, a.d.row_base + blockIdx.y);
 }
 
 template <typename T>
@@ -774,7 +672,8 @@ extern "C" size_t vrh_paged_decode_q8_workspace_bytes(int64_t rows, int32_t q_he
 
 int vrh_decode_rows_q8(const Q8Call& c, const int32_t* cu_q, int32_t num_seqs, int32_t expand_e,
                        int64_t rows, int32_t window, void* workspace, size_t workspace_bytes,
-                       bool one_split, hipStream_t s, const char* who) {
+                       bool one_split, hipStream_t s, const char* who, DecodeQ8Args* later,
+                       unsigned* later_blocks) {
   const int es = dtype_bytes(c.dtype);
   VRH_CHECK_ARG(es > 0, "%s: unknown dtype %d", who, c.dtype);
   VRH_CHECK_ARG(rows >= 0 && c.q_heads >= 1 && c.kv_heads >= 1 && c.q_heads % c.kv_heads == 0,
@@ -863,20 +762,27 @@ int vrh_decode_rows_q8(const Q8Call& c, const int32_t* cu_q, int32_t num_seqs, i
     const unsigned count = (unsigned)std::min<int64_t>(rows - first, kRowsPerLaunch);
     int64_t waves = count * per_row;
     if (a.compact) waves = std::min(waves, std::max<int64_t>(1, resident / a.units) * a.units);
+    // The caller merges the rows with its own partials.
+    const bool defer = later != nullptr && a.slots > 1 && count == rows;
+    if (defer) {
+      *later = a;
+      *later_blocks = (unsigned)(ceil_div(c.q_heads * (a.slots <= kGroup ? 1 : 4), 4) * rows);
+    }
+    const bool merge = a.slots > 1 && !defer;
     switch (c.dtype) {
       case VRH_DTYPE_F32:
         launch_valu<float>(cache_aligned(16), cache_aligned(4), (unsigned)waves, s, a);
-        if (a.slots > 1) launch_merge_q8<float>(count, s, a);
+        if (merge) launch_merge_q8<float>(count, s, a);
         break;
       case VRH_DTYPE_F16:
         if (mfma) launch_mfma_q8<f16_t>((unsigned)waves, s, a);
         else launch_valu<f16_t>(cache_aligned(16), cache_aligned(4), (unsigned)waves, s, a);
-        if (a.slots > 1) launch_merge_q8<f16_t>(count, s, a);
+        if (merge) launch_merge_q8<f16_t>(count, s, a);
         break;
       default:
         if (mfma) launch_mfma_q8<bf16_t>((unsigned)waves, s, a);
         else launch_valu<bf16_t>(cache_aligned(16), cache_aligned(4), (unsigned)waves, s, a);
-        if (a.slots > 1) launch_merge_q8<bf16_t>(count, s, a);
+        if (merge) launch_merge_q8<bf16_t>(count, s, a);
     }
   }
   VRH_RETURN_LAUNCH(who);

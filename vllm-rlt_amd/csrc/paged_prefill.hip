@@ -1037,8 +1037,23 @@ __attribute__((amdgpu_waves_per_eu(kWavesPerEu, kWavesPerEu))) void paged_prefil
 // knows whether any tile was split, and a launch for that alone cost batches of
 // short prompts and long decode rows 3-10 us (8 prompts of 16-64 queries and 4 rows
 // of 3000-4000 tokens 42.9 us, 34.5 without splits and in one launch).
-template <typename T, int D>
-__global__ __launch_bounds__(256) void paged_prefill_merge_kernel(PrefillArgs a, DecodeArgs rows,
+template <typename T, int ND>
+__device__ __forceinline__ void merge_rows(const DecodeArgs& rows, int block) {
+  const int per_row = ceil_div(rows.q_heads, 4);
+  decode_merge<T, ND>(rows, block % per_row, block / per_row);
+}
+template <typename T, int ND>
+__device__ __forceinline__ void merge_rows(const DecodeQ8Args& rows, int block) {
+  if (rows.slots <= kGroup) {
+    const int per_row = ceil_div(rows.d.q_heads, 4);
+    merge_q8<T, ND, 1>(rows, block % per_row, block / per_row);
+  } else {
+    merge_q8<T, ND, 4>(rows, block % rows.d.q_heads, block / rows.d.q_heads);
+  }
+}
+
+template <typename T, int D, typename Rows>
+__global__ __launch_bounds__(256) void paged_prefill_merge_kernel(PrefillArgs a, Rows rows,
                                                                   int decode_blocks) {
   constexpr int DB = D / 32;
   constexpr int kAhead = 4;
@@ -1046,8 +1061,7 @@ __global__ __launch_bounds__(256) void paged_prefill_merge_kernel(PrefillArgs a,
   const int gi = threadIdx.x >> 6;
   const int col = lane & 31, half = lane >> 5;
   if ((int)blockIdx.x < decode_blocks) {
-    const int per_row = ceil_div(rows.q_heads, 4);
-    decode_merge<T, (D + 63) / 64>(rows, (int)blockIdx.x % per_row, (int)blockIdx.x / per_row);
+    merge_rows<T, (D + 63) / 64>(rows, (int)blockIdx.x);
     return;
   }
   if (*a.any_split == 0) return;
@@ -1112,14 +1126,14 @@ __global__ __launch_bounds__(256) void paged_prefill_merge_kernel(PrefillArgs a,
       u32x2{pack2<T>(acc[0] * inv, acc[1] * inv), pack2<T>(acc[2] * inv, acc[3] * inv)};
 }
 
-template <typename T>
+template <typename T, typename Rows>
 bool launch_prefill_merge(int d, unsigned tile_blocks, hipStream_t s, const PrefillArgs& a,
-                          const DecodeArgs& rows, unsigned decode_blocks) {
+                          const Rows& rows, unsigned decode_blocks) {
   const dim3 grid(tile_blocks + decode_blocks);
   switch (d) {
 #define VRH_D(DV)                                                                               \
   case DV:                                                                                      \
-    hipLaunchKernelGGL((paged_prefill_merge_kernel<T, DV>), grid, dim3(256), 0, s, a, rows,     \
+    hipLaunchKernelGGL((paged_prefill_merge_kernel<T, DV, Rows>), grid, dim3(256), 0, s, a, rows,     \
                        (int)decode_blocks);                                                     \
     return true;
     VRH_D(32)
@@ -1294,7 +1308,7 @@ struct TileCall {
 
 // launch_rows(expand_e, later, later_blocks) launches the decode rows of sequences with
 // at most expand_e queries; with `later` their merge may be left to the tiles'.
-template <typename Rows>
+template <typename RowArgs, typename Rows>
 int run_tiles(const TileCall& c, hipStream_t s, Rows&& launch_rows) {
   const int dtype = c.dtype;
   const int64_t num_seqs = c.num_seqs, total_q = c.total_q;
@@ -1382,7 +1396,7 @@ int run_tiles(const TileCall& c, hipStream_t s, Rows&& launch_rows) {
             : (c.q8 ? launch_prefill<f16_t, e4m3_t>(head_dim, grid, s, a) : launch_prefill<f16_t>(head_dim, grid, s, a));
     VRH_CHECK_ARG(ok, "%s: no kernel for head_dim %d", c.who, head_dim);
   }
-  DecodeArgs rows = {};  // merged with the tiles' runs when the call may have any
+  RowArgs rows = {};  // merged with the tiles' runs when the call may have any
   unsigned decode_blocks = 0;
   if (route_rows) {
     const int rc = launch_rows(route_q, a.splits > 1 ? &rows : nullptr, &decode_blocks);
@@ -1483,7 +1497,7 @@ extern "C" int vrh_paged_prefill(int dtype, void* out, const void* q, const void
   c.workspace_bytes = workspace_bytes;
   // Short sequences of the packed batch: one split-KV decode row per query (row r is
   // query r % E of sequence r / E).
-  return run_tiles(c, s, [&](int e, DecodeArgs* later, unsigned* later_blocks) {
+  return run_tiles<DecodeArgs>(c, s, [&](int e, DecodeArgs* later, unsigned* later_blocks) {
     return vrh_decode_rows(
         dtype, out, q, key_cache, value_cache, block_tables, context_lengths, cu_seqlens_q,
         (int32_t)num_seqs, e, num_seqs * e, q_heads, kv_heads, head_dim, block_size, table_width,
@@ -1612,8 +1626,8 @@ extern "C" int vrh_paged_prefill_q8(int dtype, void* out, const void* q, const v
   t.rows_bytes = rows_bytes;
   t.workspace = workspace;
   t.workspace_bytes = workspace_bytes;
-  return run_tiles(t, s, [&](int e, DecodeArgs*, unsigned*) {
+  return run_tiles<DecodeQ8Args>(t, s, [&](int e, DecodeQ8Args* later, unsigned* later_blocks) {
     return vrh_decode_rows_q8(c, cu_seqlens_q, (int32_t)num_seqs, e, num_seqs * e, 0, workspace, rows_bytes,
-                              false, s, who);
+                              false, s, who, later, later_blocks);
   });
 }
