@@ -215,6 +215,9 @@ DECODES = [
     (torch.bfloat16, 3, 1, 33, 1, "head", 0, [40, 1]),
     (torch.bfloat16, 2, 2, 128, 128, "head", 50, [1, 128, 129, 600]),
     (torch.bfloat16, 2, 1, 128, 24, "head", 0, [1, 24, 25, 500]),
+    (torch.float32, 40, 2, 128, 16, "token", 100, [1, 100, 101, 700]),
+    (torch.float32, 16, 16, 64, 64, "head", 0, [1, 0, 63, 65, 2500]),
+    (torch.float32, 6, 3, 128, 24, "head", 0, [1, 24, 25, 500]),
 ]
 
 

@@ -205,6 +205,8 @@ struct MfmaQ8<bf16_t> {
   }
 };
 template <>
+struct MfmaQ8<float> : MfmaQ8<bf16_t> {};  // in bf16 pieces
+template <>
 struct MfmaQ8<f16_t> {
   __device__ static q8_u32x4 widen(uint32_t lo, uint32_t hi, float s0, float s1) {
     return q8_u32x4{

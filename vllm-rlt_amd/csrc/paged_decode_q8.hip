@@ -119,7 +119,9 @@ __device__ __forceinline__ bool q8_next(const DecodeQ8Args& a, uint32_t step, Wa
 // elements each (ND vectors of VE, LPT * VE apart, where that is not enough), so a
 // wave load covers 64 / LPT tokens; U such loads of K and of V are issued back to
 // back. Each token group keeps its own softmax state, merged once per split. All
-// arithmetic is fp32: float32 queries, and every shape the matrix kernel does not take.
+// arithmetic is fp32. For the shapes that the matrix kernel does not take: other head
+// dims, block sizes and alignments. It reads a KV head once per q head (37 rows of
+// 300-6000 tokens, 32 over 8 heads, 187 us against 48 of the matrix kernel).
 template <typename T, int VE, int LPT, int ND>
 __global__ __launch_bounds__(64) void paged_decode_q8_kernel(DecodeQ8Args a) {
   constexpr int U = VE >= 16 ? 8 : VE >= 4 ? 4 : 2;
@@ -276,7 +278,7 @@ __global__ __launch_bounds__(64) void paged_decode_q8_kernel(DecodeQ8Args a) {
   }
 }
 
-// ------------------------------------------------ 16-bit queries on MFMA
+// ------------------------------------------------------------- on MFMA
 // One wave per (split, KV head, row) serves up to 16 q heads of the KV head (the
 // columns of v_mfma_f32_16x16x32; groups of more take several waves):
 //  * K and V come in chunks of 32 tokens straight into a ring of kStages wave-private
@@ -290,11 +292,16 @@ __global__ __launch_bounds__(64) void paged_decode_q8_kernel(DecodeQ8Args a) {
 //  * O^T += V^T P^T per 32 tokens: the S accumulators, rounded to the query's type, are
 //    the P^T operand; one ds_read_b64_tr_b8 returns 8 tokens of a dim for V^T, whose
 //    conversion applies the page's scale (exact in bf16; in f16 see v_scale).
+//  * float32 queries and weights are three bf16 pieces each (24 bits: nothing is rounded),
+//    three MFMAs for one, while K and V are exact in bf16 already: 17 rows of 1500-2600
+//    tokens (32 over 8 heads, D = 64) 39 us in the VALU kernel, 16 here; 16 rows of about
+//    1900 tokens (16 x 64 heads) 22 and 18.
 //  * A row of LDS is D bytes of 16-byte chunks, chunk c of row r stored at slot
 //    c ^ swizzle(r), so that both readers spread over all banks.
-// A stage is 8 KiB at head_dim 128: two of them leave nine waves to a CU, more than two to
-// a SIMD, and it is other waves that cover a chunk's chain of LDS reads, MFMAs and
-// exponentials (about 1800 cycles). Three stages and six waves: 64 rows of 512-4096 tokens
+// A stage is 8 KiB at head_dim 128: two of them leave nine waves to a CU, and it is other
+// waves that cover a chunk's chain of LDS reads, MFMAs and exponentials (about 1800
+// cycles). Asked for three waves a SIMD the compiler keeps the accumulators out of AGPRs
+// and needs 127 registers (165 with float32) instead of 171. Three stages and six waves: 64 rows of 512-4096 tokens
 // (16 x 128 heads) 112 us instead of 110, 37 float16 rows of 32 over 8 heads 51 instead of
 // 48, 24 rows with a window of 1024 23.6 instead of 20.4. Without the arithmetic those 64
 // rows take 101 us (6.0 TB/s), without the loads 75.
@@ -335,8 +342,28 @@ __device__ __forceinline__ float readlane_f32(float x, int lane) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane));
 }
 
+// Two floats as three bf16 pairs each that sum to them: sink(piece, pair). A float has 24
+// significant bits and a piece takes the next 8, so nothing is rounded.
+template <typename Sink>
+__device__ __forceinline__ void split3(float a, float b, Sink sink) {
+#pragma unroll
+  for (int piece = 0; piece < 3; ++piece) {
+    const uint32_t ta = __float_as_uint(a) & 0xFFFF0000u, tb = __float_as_uint(b) & 0xFFFF0000u;
+    sink(piece, ta >> 16 | tb);
+    a -= __uint_as_float(ta);
+    b -= __uint_as_float(tb);
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void store4(T* p, f32x4_t x) {
+  if constexpr (sizeof(T) == 4) *reinterpret_cast<f32x4_t*>(p) = x;
+  else *reinterpret_cast<u32x2_t*>(p) = u32x2_t{pack2<T>(x[0], x[1]), pack2<T>(x[2], x[3])};
+}
+
 template <typename T, int D>
-__global__ __launch_bounds__(64) void paged_decode_q8_mfma_kernel(DecodeQ8Args a) {
+__global__ __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(sizeof(T) == 4 ? 2 : 3))) void
+paged_decode_q8_mfma_kernel(DecodeQ8Args a) {
   constexpr int KCH = D / 16;        // 16-byte chunks per row
   constexpr int RPI = 64 / KCH;      // rows per load instruction (8 or 16)
   constexpr int IPS = 16 / RPI;      // load instructions per 16-token step
@@ -345,6 +372,7 @@ __global__ __launch_bounds__(64) void paged_decode_q8_mfma_kernel(DecodeQ8Args a
   constexpr int DT = D / 16;         // 16-dim tiles of O^T
   constexpr int kStage = 2 * kChunk * D;
   constexpr bool kF16 = std::is_same<T, f16_t>::value;
+  constexpr int kPieces = sizeof(T) == 4 ? 3 : 1;
   __shared__ __attribute__((aligned(256))) uint8_t stage[kStages * kStage + 4 * kSegment];
   const int lane = threadIdx.x;
   const int col = lane & 15, grp = lane >> 4;
@@ -391,7 +419,7 @@ __global__ __launch_bounds__(64) void paged_decode_q8_mfma_kernel(DecodeQ8Args a
     if (n <= 0) {
       if (n == 0 && it.split == 0 && hcol) {
 #pragma unroll
-        for (int t = 0; t < DT; ++t) *reinterpret_cast<u32x2_t*>(out + 16 * t) = u32x2_t{0u, 0u};
+        for (int t = 0; t < DT; ++t) store4(out + 16 * t, f32x4_t{0.f, 0.f, 0.f, 0.f});
       }
       continue;
     }
@@ -404,7 +432,7 @@ __global__ __launch_bounds__(64) void paged_decode_q8_mfma_kernel(DecodeQ8Args a
     int ids = s0 + lane < min(s1, s0 + kSegment) ? table[s0 + lane] : 0;
 
     // Q^T operands of k-step (c, i): dims 64 c + 16 grp + 8 i .. + 7.
-    u32x4_t qop[KC][2];
+    u32x4_t qop[KC][2][kPieces];
     {
       const T* qp = reinterpret_cast<const T*>(a.d.q) + it.qrow * a.d.q_row +
                     (int64_t)(head0 + (hcol ? col : 0)) * a.d.q_head + 16 * grp;
@@ -412,8 +440,21 @@ __global__ __launch_bounds__(64) void paged_decode_q8_mfma_kernel(DecodeQ8Args a
       for (int c = 0; c < KC; ++c)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          const u32x4_t x = *reinterpret_cast<const u32x4_t*>(qp + 64 * c + 8 * i);
-          qop[c][i] = hcol ? x : u32x4_t{0u, 0u, 0u, 0u};
+          constexpr int W = (int)sizeof(T) / 2;  // 16-byte loads
+          u32x4_t x[W];
+#pragma unroll
+          for (int w = 0; w < W; ++w) {
+            x[w] = *reinterpret_cast<const u32x4_t*>(qp + 64 * c + 8 * i + 4 * w);
+            x[w] = hcol ? x[w] : u32x4_t{0u, 0u, 0u, 0u};
+          }
+          if constexpr (kPieces == 1) {
+            qop[c][i][0] = x[0];
+          } else {
+#pragma unroll
+            for (int w = 0; w < 4; ++w)
+              split3(__uint_as_float(x[w / 2][2 * w % 4]), __uint_as_float(x[w / 2][2 * w % 4 + 1]),
+                     [&](int piece, uint32_t pair) { qop[c][i][piece][w] = pair; });
+          }
         }
     }
 
@@ -490,8 +531,13 @@ __global__ __launch_bounds__(64) void paged_decode_q8_mfma_kernel(DecodeQ8Args a
 #pragma unroll
           for (int c = 0; c < KC; ++c) {
             const u32x4_t x = lds_read16(koff[t][c] + st * kStage);
-            sc[t] = MfmaQ8<T>::run(MfmaQ8<T>::widen(x[0], x[1], 1.f, 1.f), qop[c][0], sc[t]);
-            sc[t] = MfmaQ8<T>::run(MfmaQ8<T>::widen(x[2], x[3], 1.f, 1.f), qop[c][1], sc[t]);
+            const u32x4_t lo = MfmaQ8<T>::widen(x[0], x[1], 1.f, 1.f);
+            const u32x4_t hi = MfmaQ8<T>::widen(x[2], x[3], 1.f, 1.f);
+#pragma unroll
+            for (int w = 0; w < kPieces; ++w) {
+              sc[t] = MfmaQ8<T>::run(lo, qop[c][0][w], sc[t]);
+              sc[t] = MfmaQ8<T>::run(hi, qop[c][1][w], sc[t]);
+            }
           }
         }
         // Scales of the chunk's two 16-token tiles (the second may lie past the last page).
@@ -538,12 +584,21 @@ __global__ __launch_bounds__(64) void paged_decode_q8_mfma_kernel(DecodeQ8Args a
 #pragma unroll
             for (int i = 0; i < 4; ++i) p[t][i] *= ps[t];
         }
-        const u32x4_t pop = u32x4_t{pack2<T>(p[0][0], p[0][1]), pack2<T>(p[0][2], p[0][3]),
-                                    pack2<T>(p[1][0], p[1][1]), pack2<T>(p[1][2], p[1][3])};
+        u32x4_t pop[kPieces];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (kPieces == 1)
+            pop[0][i] = pack2<T>(p[i / 2][2 * (i & 1)], p[i / 2][2 * (i & 1) + 1]);
+          else
+            split3(p[i / 2][2 * (i & 1)], p[i / 2][2 * (i & 1) + 1],
+                   [&](int piece, uint32_t pair) { pop[piece][i] = pair; });
+        }
 #pragma unroll
         for (int t = 0; t < DT; ++t) {
           const u32x2_t x = lds_tr8(voff[t] + st * kStage);
-          acc[t] = MfmaQ8<T>::run(MfmaQ8<T>::widen(x[0], x[1], vs[0], vs[1]), pop, acc[t]);
+          const u32x4_t v = MfmaQ8<T>::widen(x[0], x[1], vs[0], vs[1]);
+#pragma unroll
+          for (int w = 0; w < kPieces; ++w) acc[t] = MfmaQ8<T>::run(v, pop[w], acc[t]);
         }
       };
       // Step j: chunk j has landed (only the loads of later chunks may be in flight); the
@@ -581,8 +636,7 @@ __global__ __launch_bounds__(64) void paged_decode_q8_mfma_kernel(DecodeQ8Args a
       const float inv = 1.f / lsum;
 #pragma unroll
       for (int t = 0; t < DT; ++t)
-        *reinterpret_cast<u32x2_t*>(out + 16 * t) =
-            u32x2_t{pack2<T>(acc[t][0] * inv, acc[t][1] * inv), pack2<T>(acc[t][2] * inv, acc[t][3] * inv)};
+        store4(out + 16 * t, acc[t] * inv);
       continue;
     }
     const int64_t idx = (it.row * a.d.q_heads + head0 + col) * a.slots + it.split;
@@ -733,14 +787,14 @@ int vrh_decode_rows_q8(const Q8Call& c, const int32_t* cu_q, int32_t num_seqs, i
     return c.head_dim % v == 0 && c.c_block % v == 0 && c.c_token % v == 0 && c.c_head % v == 0 &&
            (uintptr_t)c.k % v == 0 && (uintptr_t)c.v % v == 0;
   };
-  // The matrix kernel: 16-bit queries, head_dim 64 or 128, blocks of a power of two of
+  // The matrix kernel: head_dim 64 or 128, blocks of a power of two of
   // tokens from 16 on, 16-byte aligned rows, scale pairs that do not straddle a word, row offsets
   // within a load instruction in 32 bits.
-  const bool mfma = c.dtype != VRH_DTYPE_F32 && (c.head_dim == 64 || c.head_dim == 128) &&
+  const bool mfma = (c.head_dim == 64 || c.head_dim == 128) &&
                     a.d.bs_shift >= 4 && c.block_size <= 65536 && cache_aligned(16) && c.c_token < (1 << 26) &&
-                    c.c_token >= 0 && c.c_block >= 0 && c.q_row % 8 == 0 && c.q_head % 8 == 0 &&
-                    c.o_row % 4 == 0 && c.o_head % 4 == 0 && (uintptr_t)c.q % 16 == 0 &&
-                    (uintptr_t)c.out % 8 == 0 && c.s_block % 2 == 0 && c.s_head % 2 == 0 &&
+                    c.c_token >= 0 && c.c_block >= 0 && c.q_row * es % 16 == 0 &&
+                    c.q_head * es % 16 == 0 && c.o_row % 4 == 0 && c.o_head % 4 == 0 &&
+                    (uintptr_t)c.q % 16 == 0 && (uintptr_t)c.out % (4 * es) == 0 && c.s_block % 2 == 0 && c.s_head % 2 == 0 &&
                     (uintptr_t)c.scales % 2 == 0;
   a.tiles = mfma ? ceil_div(a.d.group, 16) : 1;
   a.units = mfma ? c.kv_heads * a.tiles : c.q_heads;
@@ -771,7 +825,8 @@ int vrh_decode_rows_q8(const Q8Call& c, const int32_t* cu_q, int32_t num_seqs, i
     const bool merge = a.slots > 1 && !defer;
     switch (c.dtype) {
       case VRH_DTYPE_F32:
-        launch_valu<float>(cache_aligned(16), cache_aligned(4), (unsigned)waves, s, a);
+        if (mfma) launch_mfma_q8<float>((unsigned)waves, s, a);
+        else launch_valu<float>(cache_aligned(16), cache_aligned(4), (unsigned)waves, s, a);
         if (merge) launch_merge_q8<float>(count, s, a);
         break;
       case VRH_DTYPE_F16:
