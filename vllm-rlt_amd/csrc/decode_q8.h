@@ -223,7 +223,8 @@ struct MfmaQ8<f16_t> {
 
 // Softmax weights are rounded to the query's type for the V product: exp2(s - m) where
 // the reference m was the largest score minus kLift when it last moved, and moves when
-// a score passes it by kSlack. bf16 rounds every weight by at most 2^-9 of it. f16 has
+// a score passes it by kSlack. bf16 rounds every weight by at most 2^-8 of it (half a step;
+// float32 weights are split into exact pieces instead). f16 has
 // few exponents: lifted by 2^7 its weights go down to 2^-21 of the largest before they
 // get subnormal (2^-14 unlifted), and up to 2^12 (2^15 with the factor of v_scale).
 template <typename T>

@@ -107,7 +107,8 @@ __device__ __forceinline__ void sequence_request(const SequenceArgs& a, int64_t 
 // Workgroups [0, n): one request each (its table row, length and cumulative count);
 // the others 256 tokens each. Every workgroup scans the counts itself, 1024 requests
 // at a time: a scan of its own launch would cost more than reading 12 bytes a request
-// from L2 again.
+// from L2 again. Bound by latency (two dependent misses and the scan): 64 requests of
+// 8000 tokens 4.6 us, 500 requests under tables of 2048 pages (6 MB) 5.7 us.
 __global__ __launch_bounds__(256) void sequence_metadata_kernel(SequenceArgs a) {
   __shared__ int64_t ends[kScan];  // where each request's tokens end
   __shared__ int64_t wave_total[4];

@@ -7,6 +7,10 @@
 // keys are cut into splits of whole pages whose (max, sum, accumulator) are merged
 // in split order. The cut depends on the row's own length only, so a row's result
 // does not depend on the batch, and a packed query equals a decode row bit for bit.
+//
+// Bound by HBM: 2 bytes per visible token, KV head and dim. 64 rows of 512-4096 tokens
+// (16 x 128 heads, bf16, 607 MB): 107 us, 5.7 TB/s, and 5 us of merge. Lone rows and short
+// ones are bound by latency: length, page ids, K and V, merge.
 #include <algorithm>
 #include <type_traits>
 
